@@ -13,7 +13,9 @@
 #include <signal.h>
 #include <unistd.h>
 
+#include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdlib>
 #include <string>
 #include <vector>
@@ -744,6 +746,234 @@ std::vector<int64_t> status_record() {
   return {w[0], w[1], q[1], q[2]};
 }
 
+// ---------------------------------------------------------------- long-text operators
+// These allocate their outputs here: their smallest calls (one token) are as
+// short as the allocations.
+int elem_type(const at::Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return ewb::kElemBf16;
+    case at::kHalf: return ewb::kElemF16;
+    case at::kFloat: return ewb::kElemF32;
+    default: TORCH_CHECK(false, name, " must be bf16, fp16 or fp32"); return -1;
+  }
+}
+
+int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+void check_inner(const at::Tensor& t, const char* name) {
+  check_cuda(t, name);
+  TORCH_CHECK(t.dim() == 2, name, " must be 2-D");
+  TORCH_CHECK(t.size(1) <= 1 || t.stride(1) == 1, name, " must have a contiguous inner dimension");
+}
+
+void check_same_device(const at::Tensor& t, const at::Tensor& as, const char* name) {
+  TORCH_CHECK(t.device() == as.device(), name, " must be on ", as.device());
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+at::Tensor dropout_add(at::Tensor x, c10::optional<at::Tensor> resid, double p, uint64_t seed,
+                       uint64_t stream, c10::optional<at::ScalarType> out_dtype) {
+  check_inner(x, "x");
+  TORCH_CHECK(p >= 0.0 && p < 1.0, "dropout: p must be in [0, 1)");
+  c10::cuda::CUDAGuard guard(x.device());
+  ewb::DropoutArgs a{};
+  a.rows = x.size(0);
+  a.d = x.size(1);
+  a.x = x.data_ptr();
+  a.ldx = row_stride(x);
+  a.x_type = elem_type(x, "x");
+  TORCH_CHECK(a.x_type != ewb::kElemF16, "x must be bf16 or fp32");
+  if (resid.has_value() && resid->defined()) {
+    check_same_device(*resid, x, "resid");
+    check_inner(*resid, "resid");
+    TORCH_CHECK(resid->sizes() == x.sizes(), "resid must have x's shape");
+    a.resid = resid->data_ptr();
+    a.ldr = row_stride(*resid);
+    a.resid_type = elem_type(*resid, "resid");
+  }
+  at::Tensor y = at::empty({a.rows, a.d}, x.options().dtype(out_dtype.value_or(x.scalar_type())));
+  a.y = y.data_ptr();
+  a.ldy = a.d;
+  a.y_type = elem_type(y, "out_dtype");
+  const double t = std::nearbyint(p * 4294967296.0);
+  a.thr = t >= 4294967295.0 ? 0xffffffffu : static_cast<uint32_t>(t);
+  a.scale = static_cast<float>(1.0 / (1.0 - p));
+  a.seed = seed;
+  a.stream = stream;
+  ok(ewb::dropout_add(a, cur_stream()), "dropout_add");
+  if (x.numel() > 0) count(1);
+  return y;
+}
+
+const int64_t* checked_targets(const c10::optional<at::Tensor>& targets, const at::Tensor& logits) {
+  if (!targets.has_value() || !targets->defined()) return nullptr;
+  check_same_device(*targets, logits, "targets");
+  TORCH_CHECK(targets->scalar_type() == at::kLong && targets->is_contiguous() &&
+                  targets->numel() == logits.size(0),
+              "targets must be int64, one for each row");
+  return targets->data_ptr<int64_t>();
+}
+
+std::vector<c10::optional<at::Tensor>> token_logprobs(at::Tensor logits, int64_t V,
+                                                      c10::optional<at::Tensor> targets, int64_t top) {
+  check_inner(logits, "logits");
+  TORCH_CHECK(V >= 1 && V <= logits.size(1) && V < 0x7fff0000, "logits must have V columns");
+  TORCH_CHECK(top >= 0 && top <= 32 && top <= V, "top must be in [0, 32] and no more than V");
+  c10::cuda::CUDAGuard guard(logits.device());
+  ewb::LogprobsArgs a{};
+  a.logits = logits.data_ptr();
+  a.ld = row_stride(logits);
+  a.type = elem_type(logits, "logits");
+  TORCH_CHECK(a.type != ewb::kElemF16, "logits must be bf16 or fp32");
+  a.rows = logits.size(0);
+  a.V = static_cast<int>(V);
+  a.targets = checked_targets(targets, logits);
+  a.top = static_cast<int>(top);
+  const auto f32 = logits.options().dtype(at::kFloat);
+  c10::optional<at::Tensor> logp, top_logp, top_ids;
+  at::Tensor entropy = at::empty({a.rows}, f32), lse = at::empty({a.rows}, f32);
+  if (a.targets != nullptr) logp = at::empty({a.rows}, f32);
+  if (top > 0) {
+    top_logp = at::empty({a.rows, top}, f32);
+    top_ids = at::empty({a.rows, top}, logits.options().dtype(at::kLong));
+  }
+  a.logp = logp ? logp->data_ptr<float>() : nullptr;
+  a.entropy = entropy.data_ptr<float>();
+  a.lse = lse.data_ptr<float>();
+  a.top_logp = top_logp ? top_logp->data_ptr<float>() : nullptr;
+  a.top_ids = top_ids ? top_ids->data_ptr<int64_t>() : nullptr;
+  a.status = status_word(logits.get_device());
+  ok(ewb::token_logprobs(a, cur_stream()), "token_logprobs");
+  if (a.rows > 0) count(1);
+  return {logp, entropy, lse, top_logp, top_ids};
+}
+
+const float* checked_rows(const c10::optional<at::Tensor>& t, const at::Tensor& logits, const char* name) {
+  if (!t.has_value() || !t->defined()) return nullptr;
+  check_same_device(*t, logits, name);
+  TORCH_CHECK(t->scalar_type() == at::kFloat && t->is_contiguous() && t->numel() == logits.size(0), name,
+              " must be fp32, one for each row");
+  return t->data_ptr<float>();
+}
+
+at::Tensor token_logprobs_bwd(at::Tensor logits, int64_t V, c10::optional<at::Tensor> targets,
+                              at::Tensor lse, at::Tensor entropy, c10::optional<at::Tensor> g_logp,
+                              c10::optional<at::Tensor> g_entropy, int64_t ld_grad,
+                              at::ScalarType out_dtype) {
+  check_inner(logits, "logits");
+  TORCH_CHECK(V >= 1 && V <= logits.size(1), "logits must have V columns");
+  TORCH_CHECK(ld_grad >= V && ld_grad < 0x7fff0000, "ld_grad must be at least V");
+  c10::cuda::CUDAGuard guard(logits.device());
+  ewb::LogprobsBwdArgs a{};
+  a.logits = logits.data_ptr();
+  a.ld = row_stride(logits);
+  a.type = elem_type(logits, "logits");
+  TORCH_CHECK(a.type != ewb::kElemF16, "logits must be bf16 or fp32");
+  a.rows = logits.size(0);
+  a.V = static_cast<int>(V);
+  a.targets = checked_targets(targets, logits);
+  a.lse = checked_rows(lse, logits, "lse");
+  a.entropy = checked_rows(entropy, logits, "entropy");
+  a.g_logp = checked_rows(g_logp, logits, "g_logp");
+  a.g_entropy = checked_rows(g_entropy, logits, "g_entropy");
+  TORCH_CHECK(a.lse != nullptr && a.entropy != nullptr, "lse and entropy of the forward are needed");
+  at::Tensor grad = at::empty({a.rows, ld_grad}, logits.options().dtype(out_dtype));
+  a.grad = grad.data_ptr();
+  a.ldg = a.cols = ld_grad;
+  a.grad_type = elem_type(grad, "out_dtype");
+  TORCH_CHECK(a.grad_type != ewb::kElemF16, "out_dtype must be bf16 or fp32");
+  ok(ewb::token_logprobs_bwd(a, cur_stream()), "token_logprobs_bwd");
+  if (a.rows > 0) count(1);
+  return grad;
+}
+
+// The shape rules that every window attention call shares.
+void check_window(const at::Tensor& qkv, int64_t H, int64_t hd, int64_t Hkv, int64_t window,
+                  int64_t sinks) {
+  check_inner(qkv, "qkv");
+  TORCH_CHECK(qkv.scalar_type() == at::kBFloat16, "qkv must be bf16");
+  TORCH_CHECK(hd == 64 || hd == 80 || hd == 96 || hd == 128, "head width must be 64, 80, 96 or 128, got ", hd);
+  TORCH_CHECK(H >= 1 && Hkv >= 1 && H % Hkv == 0, "H must be a multiple of Hkv");
+  TORCH_CHECK(qkv.size(1) == (H + 2 * Hkv) * hd, "qkv rows must hold q | k | v: ", (H + 2 * Hkv) * hd,
+              " columns, got ", qkv.size(1));
+  TORCH_CHECK(aligned16(qkv.data_ptr()) && row_stride(qkv) % 8 == 0, "qkv rows must be 16-byte aligned");
+  TORCH_CHECK(window >= 1 && sinks >= 0, "window must be at least 1 and sinks at least 0");
+}
+
+const int* checked_lengths(const c10::optional<at::Tensor>& lengths, const at::Tensor& qkv, int64_t B) {
+  if (!lengths.has_value() || !lengths->defined()) return nullptr;
+  check_same_device(*lengths, qkv, "lengths");
+  TORCH_CHECK(lengths->scalar_type() == at::kInt && lengths->is_contiguous() && lengths->numel() == B,
+              "lengths must be int32, one for each sequence");
+  return lengths->data_ptr<int>();
+}
+
+void check_ring(const at::Tensor& cache, const at::Tensor& qkv, int64_t B, int64_t Hkv, int64_t hd,
+                int64_t sinks) {
+  check_same_device(cache, qkv, "cache");
+  TORCH_CHECK(cache.dim() == 3 && cache.size(0) == B && cache.size(2) == 2 * Hkv * hd && cache.stride(2) == 1,
+              "cache must be [B, slots, 2 * Hkv * hd]");
+  TORCH_CHECK(cache.scalar_type() == at::kBFloat16, "cache must be bf16");
+  TORCH_CHECK(cache.size(1) > sinks && cache.size(1) < 0x7fffffff, "cache must have more slots than sinks");
+  TORCH_CHECK(aligned16(cache.data_ptr()) && cache.stride(0) % 8 == 0 && cache.stride(1) % 8 == 0,
+              "cache rows must be 16-byte aligned");
+}
+
+at::Tensor window_step(at::Tensor qkv, at::Tensor cache, at::Tensor pos, int64_t H, int64_t hd,
+                       int64_t Hkv, int64_t window, int64_t sinks, double scale) {
+  check_window(qkv, H, hd, Hkv, window, sinks);
+  const int64_t B = qkv.size(0);
+  check_ring(cache, qkv, B, Hkv, hd, sinks);
+  check_same_device(pos, qkv, "pos");
+  TORCH_CHECK(pos.scalar_type() == at::kLong && pos.is_contiguous() && pos.numel() == B,
+              "pos must be int64, one for each sequence");
+  c10::cuda::CUDAGuard guard(qkv.device());
+  at::Tensor o = at::empty({B, H * hd}, qkv.options());
+  ewb::WindowStepArgs a{};
+  a.qkv = reinterpret_cast<const __nv_bfloat16*>(qkv.data_ptr());
+  a.ldq = row_stride(qkv);
+  a.cache = reinterpret_cast<__nv_bfloat16*>(cache.data_ptr());
+  a.stride_b = cache.stride(0);
+  a.stride_s = cache.stride(1);
+  a.pos = pos.data_ptr<int64_t>();
+  a.o = reinterpret_cast<__nv_bfloat16*>(o.data_ptr());
+  a.B = B;
+  a.H = H;
+  a.Hkv = Hkv;
+  a.hd = hd;
+  a.window = static_cast<int>(std::min<int64_t>(window, 0x7fffffff));
+  a.sinks = sinks;
+  a.cap = cache.size(1);
+  a.scale = static_cast<float>(scale);
+  ok(ewb::window_step(a, cur_stream()), "window_step");
+  if (B > 0) count(1);
+  return o;
+}
+
+void window_fill(at::Tensor qkv, at::Tensor cache, int64_t B, int64_t S, int64_t H, int64_t hd,
+                 int64_t Hkv, int64_t sinks, c10::optional<at::Tensor> lengths) {
+  check_window(qkv, H, hd, Hkv, 1, sinks);
+  TORCH_CHECK(B >= 0 && S >= 0 && qkv.size(0) == B * S, "qkv must have B * S rows");
+  check_ring(cache, qkv, B, Hkv, hd, sinks);
+  c10::cuda::CUDAGuard guard(qkv.device());
+  ewb::WindowFillArgs a{};
+  a.qkv = reinterpret_cast<const __nv_bfloat16*>(qkv.data_ptr());
+  a.ldq = row_stride(qkv);
+  a.kv_col = H * hd;
+  a.width = 2 * Hkv * hd;
+  a.cache = reinterpret_cast<__nv_bfloat16*>(cache.data_ptr());
+  a.stride_b = cache.stride(0);
+  a.stride_s = cache.stride(1);
+  a.lengths = checked_lengths(lengths, qkv, B);
+  a.B = B;
+  a.S = S;
+  a.sinks = sinks;
+  a.cap = cache.size(1);
+  ok(ewb::window_fill(a, cur_stream()), "window_fill");
+  if (B * S > 0) count(1);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -765,6 +995,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("layernorm_bwd_chunks", &layernorm_bwd_chunks);
   m.def("attention_fwd", &attention_fwd);
   m.def("attention_bwd", &attention_bwd);
+  m.def("dropout_add", &dropout_add);
+  m.def("token_logprobs", &token_logprobs);
+  m.def("token_logprobs_bwd", &token_logprobs_bwd);
+  m.def("window_step", &window_step);
+  m.def("window_fill", &window_fill);
   m.def("rope", &rope);
   m.def("swiglu_fwd", &swiglu_fwd);
   m.def("swiglu_bwd", &swiglu_bwd);

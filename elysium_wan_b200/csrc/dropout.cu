@@ -1,0 +1,251 @@
+// Dropout on a residual branch: y = resid + x * keep / (1 - p), and its
+// gradient dx = dy * keep / (1 - p). The mask is never stored: the backward
+// makes the same words again.
+//
+// keep(e) = word(e) >= round(p 2^32) for element e = row * d + column. The
+// words come from the counter-based generator Philox4x32-10 (Salmon, Moraes,
+// Dror, Shaw, "Parallel random numbers: as easy as 1, 2, 3", SC 2011): word e is
+// word e % 4 of the block whose 128-bit counter is (e / 4, stream) and whose
+// 64-bit key is the seed. A mask so depends on (seed, stream, element) alone:
+// not on the launch shape, the strides, the GPU or the pipeline cut.
+//
+// Bound by memory: 2 bytes read for x, 2 for the residual, 2 written (bf16).
+// A block of ten rounds is 20 wide multiplications and 20 three-input xors
+// for four elements, which is under the issue rate left by the copies.
+#include "common.cuh"
+#include "kernels.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace ewb {
+namespace {
+
+constexpr int kDropThreads = 256;
+
+struct PhiloxKey {
+  uint32_t k0, k1, s0, s1;
+};
+
+__device__ __forceinline__ uint4 philox(uint64_t block, const PhiloxKey& key) {
+  uint32_t c0 = static_cast<uint32_t>(block), c1 = static_cast<uint32_t>(block >> 32);
+  uint32_t c2 = key.s0, c3 = key.s1;
+  uint32_t k0 = key.k0, k1 = key.k1;
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    const uint64_t a = static_cast<uint64_t>(0xD2511F53u) * c0;
+    const uint64_t b = static_cast<uint64_t>(0xCD9E8D57u) * c2;
+    c0 = static_cast<uint32_t>(b >> 32) ^ c1 ^ k0;
+    c1 = static_cast<uint32_t>(b);
+    c2 = static_cast<uint32_t>(a >> 32) ^ c3 ^ k1;
+    c3 = static_cast<uint32_t>(a);
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return make_uint4(c0, c1, c2, c3);
+}
+
+// ---------------------------------------------------------------- element access
+template <typename T>
+__device__ __forceinline__ float to_f(T v);
+template <>
+__device__ __forceinline__ float to_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+
+// Eight consecutive elements, 16-byte aligned (32 bytes for fp32).
+template <typename T>
+struct Raw8 {
+  uint4 w;
+};
+template <>
+struct Raw8<float> {
+  uint4 w, w2;
+};
+
+template <typename T>
+__device__ __forceinline__ Raw8<T> load8(const T* p) {
+  Raw8<T> r;
+  r.w = __ldcs(reinterpret_cast<const uint4*>(p));
+  if constexpr (sizeof(T) == 4) r.w2 = __ldcs(reinterpret_cast<const uint4*>(p) + 1);
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack8(const Raw8<T>& r, float* v) {
+  if constexpr (sizeof(T) == 4) {
+    const uint32_t u[8] = {r.w.x, r.w.y, r.w.z, r.w.w, r.w2.x, r.w2.y, r.w2.z, r.w2.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(u[i]);
+  } else {
+    unpack8_fmt(r.w, std::is_same<T, __half>::value ? kFmtF16 : kFmtBf16, 1.0f, v);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float* v) {
+  uint4* q = reinterpret_cast<uint4*>(p);
+  if constexpr (sizeof(T) == 4) {
+    q[0] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    q[1] = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
+  } else if constexpr (std::is_same<T, __half>::value) {
+    q[0] = make_uint4(pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3]), pack_f16x2(v[4], v[5]), pack_f16x2(v[6], v[7]));
+  } else {
+    q[0] = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+  }
+}
+
+__device__ __forceinline__ float drop(float x, uint32_t word, uint32_t thr, float scale) {
+  return word >= thr ? x * scale : 0.0f;
+}
+
+// Rows of d elements in vectors of eight (blockIdx.y walks the rows). With
+// more than one row d is a multiple of eight; one row (dense tensors are one
+// row of all their elements) may end in a tail, which the last thread takes.
+template <typename TX, typename TR, typename TY, bool kResid>
+__global__ void __launch_bounds__(kDropThreads)
+    dropout_vec_kernel(const TX* __restrict__ x, int64_t ldx, const TR* __restrict__ resid,
+                       int64_t ldr, TY* __restrict__ y, int64_t ldy, int64_t rows, int64_t d,
+                       uint32_t thr, float scale, PhiloxKey key) {
+  const int64_t nv = d >> 3;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kDropThreads;
+  for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
+    const TX* xr = x + row * ldx;
+    const TR* rr = kResid ? resid + row * ldr : nullptr;
+    TY* yr = y + row * ldy;
+    const uint64_t e0 = static_cast<uint64_t>(row) * d;
+    int64_t v = static_cast<int64_t>(blockIdx.x) * kDropThreads + threadIdx.x;
+    for (; v < nv; v += step) {
+      const Raw8<TX> rx = load8(xr + 8 * v);
+      Raw8<TR> rs;
+      if constexpr (kResid) rs = load8(rr + 8 * v);
+      const uint64_t blk = (e0 >> 2) + 2 * static_cast<uint64_t>(v);
+      const uint4 a = philox(blk, key), b = philox(blk + 1, key);
+      const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+      float f[8], g[8];
+      unpack8(rx, f);
+      if constexpr (kResid) unpack8(rs, g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        f[i] = drop(f[i], w[i], thr, scale);
+        if constexpr (kResid) f[i] += g[i];
+      }
+      store8(yr + 8 * v, f);
+    }
+    if (v == nv) {  // the thread after the last whole vector
+      for (int64_t c = 8 * nv; c < d; ++c) {
+        const uint4 a = philox((e0 + c) >> 2, key);
+        const int k = static_cast<int>((e0 + c) & 3);
+        const uint32_t w = k == 0 ? a.x : k == 1 ? a.y : k == 2 ? a.z : a.w;
+        float f = drop(to_f(xr[c]), w, thr, scale);
+        if constexpr (kResid) f += to_f(rr[c]);
+        yr[c] = from_f<TY>(f);
+      }
+    }
+  }
+}
+
+// Any strides and alignments: one thread per block of four elements, element
+// by element (a block may run over a row's end).
+template <typename TX, typename TR, typename TY, bool kResid>
+__global__ void __launch_bounds__(kDropThreads)
+    dropout_any_kernel(const TX* __restrict__ x, int64_t ldx, const TR* __restrict__ resid,
+                       int64_t ldr, TY* __restrict__ y, int64_t ldy, int64_t rows, int64_t d,
+                       uint32_t thr, float scale, PhiloxKey key) {
+  const int64_t n = rows * d, nb = (n + 3) >> 2;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kDropThreads;
+  for (int64_t b = static_cast<int64_t>(blockIdx.x) * kDropThreads + threadIdx.x; b < nb; b += step) {
+    const uint4 a = philox(static_cast<uint64_t>(b), key);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+    int64_t row = (4 * b) / d, col = 4 * b - row * d;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (4 * b + k >= n) break;
+      float f = drop(to_f(x[row * ldx + col]), w[k], thr, scale);
+      if constexpr (kResid) f += to_f(resid[row * ldr + col]);
+      y[row * ldy + col] = from_f<TY>(f);
+      if (++col == d) {
+        col = 0;
+        ++row;
+      }
+    }
+  }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <typename TX, typename TR, typename TY, bool kResid>
+int launch(const DropoutArgs& a, cudaStream_t stream) {
+  const TX* x = static_cast<const TX*>(a.x);
+  const TR* r = static_cast<const TR*>(a.resid);
+  TY* y = static_cast<TY*>(a.y);
+  const PhiloxKey key{static_cast<uint32_t>(a.seed), static_cast<uint32_t>(a.seed >> 32),
+                      static_cast<uint32_t>(a.stream), static_cast<uint32_t>(a.stream >> 32)};
+  int64_t rows = a.rows, d = a.d, ldx = a.ldx, ldr = a.ldr, ldy = a.ldy;
+  if (rows == 1 || (ldx == d && ldy == d && (!kResid || ldr == d))) {
+    d *= rows;  // dense: one long row
+    rows = 1;
+    ldx = ldy = ldr = d;
+  }
+  // 16-byte vectors need aligned bases and, from row to row, aligned steps
+  const bool bases = aligned16(x) && aligned16(y) && (!kResid || aligned16(r));
+  const bool steps = rows == 1 || (d % 8 == 0 && ldx % 8 == 0 && ldy % 8 == 0 && (!kResid || ldr % 8 == 0));
+  const int64_t most = 148 * 8;  // every resident block of an SM
+  if (bases && steps) {
+    const int64_t bx = std::max<int64_t>(1, std::min<int64_t>((d / 8 + kDropThreads) / kDropThreads, most));
+    const int64_t by = std::min<int64_t>(rows, std::max<int64_t>(1, 4 * most / bx));
+    dropout_vec_kernel<TX, TR, TY, kResid>
+        <<<dim3(static_cast<unsigned>(bx), static_cast<unsigned>(by)), kDropThreads, 0, stream>>>(
+            x, ldx, r, ldr, y, ldy, rows, d, a.thr, a.scale, key);
+  } else {
+    const int64_t bx = std::min<int64_t>((rows * d / 4 + kDropThreads) / kDropThreads, 4 * most);
+    dropout_any_kernel<TX, TR, TY, kResid><<<static_cast<unsigned>(bx), kDropThreads, 0, stream>>>(
+        x, ldx, r, ldr, y, ldy, rows, d, a.thr, a.scale, key);
+  }
+  return cudaGetLastError() == cudaSuccess ? 0 : 2;
+}
+
+template <typename TX, typename TR, bool kResid>
+int launch_y(const DropoutArgs& a, cudaStream_t stream) {
+  switch (a.y_type) {
+    case kElemBf16: return launch<TX, TR, __nv_bfloat16, kResid>(a, stream);
+    case kElemF16: return launch<TX, TR, __half, kResid>(a, stream);
+    case kElemF32: return launch<TX, TR, float, kResid>(a, stream);
+    default: return 1;
+  }
+}
+
+template <typename TX>
+int launch_r(const DropoutArgs& a, cudaStream_t stream) {
+  if (a.resid == nullptr) return launch_y<TX, __nv_bfloat16, false>(a, stream);
+  switch (a.resid_type) {
+    case kElemBf16: return launch_y<TX, __nv_bfloat16, true>(a, stream);
+    case kElemF16: return launch_y<TX, __half, true>(a, stream);
+    case kElemF32: return launch_y<TX, float, true>(a, stream);
+    default: return 1;
+  }
+}
+
+}  // namespace
+
+int dropout_add(const DropoutArgs& a, cudaStream_t stream) {
+  if (a.rows < 0 || a.d < 0) return 1;
+  if (a.rows == 0 || a.d == 0) return 0;
+  switch (a.x_type) {
+    case kElemBf16: return launch_r<__nv_bfloat16>(a, stream);
+    case kElemF32: return launch_r<float>(a, stream);
+    default: return 1;
+  }
+}
+
+}  // namespace ewb

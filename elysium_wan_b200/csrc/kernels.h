@@ -209,4 +209,113 @@ struct SwigluBwdArgs {
 };
 int swiglu_bwd(const SwigluBwdArgs& a, cudaStream_t stream);
 
+// ---------------------------------------------------------------- dropout
+enum ElemType : int { kElemBf16 = 0, kElemF16 = 1, kElemF32 = 2 };
+
+// y = resid + x * keep / (1 - p) over [rows][d]; resid may be null (the
+// gradient of x is the same map of dy). keep: word(row * d + col) >= thr.
+struct DropoutArgs {
+  const void* x;  // bf16 or fp32
+  int64_t ldx;
+  int x_type;
+  const void* resid;  // bf16, fp16 or fp32
+  int64_t ldr;
+  int resid_type;
+  void* y;  // bf16, fp16 or fp32
+  int64_t ldy;
+  int y_type;
+  int64_t rows, d;
+  uint32_t thr;  // round(p 2^32)
+  float scale;   // 1 / (1 - p)
+  uint64_t seed, stream;
+};
+int dropout_add(const DropoutArgs& a, cudaStream_t stream);
+
+// ---------------------------------------------------------------- token log probabilities
+struct LogprobsArgs {
+  const void* logits;  // [rows][ld], V valid columns, bf16 or fp32
+  int64_t ld;
+  int type;
+  int64_t rows;
+  int V;
+  const int64_t* targets;  // may be null (then logp is null too); negative = none given
+  int top;                 // alternatives, 0..32
+  float* logp;
+  float* entropy;
+  float* lse;
+  float* top_logp;   // [rows][top]
+  int64_t* top_ids;  // [rows][top]
+  int* status;       // status record: a target >= V is reported here
+};
+int token_logprobs(const LogprobsArgs& a, cudaStream_t stream);
+
+struct LogprobsBwdArgs {
+  const void* logits;
+  int64_t ld;
+  int type;
+  int64_t rows;
+  int V;
+  const int64_t* targets;
+  const float* lse;
+  const float* entropy;
+  const float* g_logp;     // may be null
+  const float* g_entropy;  // may be null
+  void* grad;              // [rows][ldg], columns [V, cols) are set to 0
+  int64_t ldg;
+  int grad_type;
+  int64_t cols;
+};
+int token_logprobs_bwd(const LogprobsBwdArgs& a, cudaStream_t stream);
+
+// ---------------------------------------------------------------- window attention, one token
+// A ring of `cap` rows of [k | v] (Hkv heads of hd each) a sequence.
+struct WindowStepArgs {
+  const __nv_bfloat16* qkv;  // [B][ldq]: the new tokens' q | k | v
+  int64_t ldq;
+  __nv_bfloat16* cache;
+  int64_t stride_b, stride_s;
+  const int64_t* pos;  // [B] position of the new token; negative = idle
+  __nv_bfloat16* o;    // [B][H * hd]
+  int64_t B;
+  int H, Hkv, hd, window, sinks, cap;
+  float scale;
+};
+int window_step(const WindowStepArgs& a, cudaStream_t stream);
+
+struct WindowFillArgs {
+  const __nv_bfloat16* qkv;  // [B * S][ldq]; k | v start at column kv_col
+  int64_t ldq;
+  int kv_col, width;  // width = 2 * Hkv * hd
+  __nv_bfloat16* cache;
+  int64_t stride_b, stride_s;
+  const int* lengths;  // [B], may be null (all S)
+  int64_t B;
+  int S, sinks, cap;
+};
+int window_fill(const WindowFillArgs& a, cudaStream_t stream);
+
+// ---------------------------------------------------------------- window attention
+// Query i sees key j <= i when i - j < window or j < sinks, and both lie below
+// the sequence's length. Rows at or past the length: o = 0, lse = -inf.
+struct WindowAttnArgs {
+  const __nv_bfloat16* qkv;  // [B * S][ldq]: q (H heads) | k (Hkv) | v (Hkv)
+  int64_t ldq;
+  __nv_bfloat16* o;  // [B * S][H * hd]
+  float* lse;        // [B][H][S] base 2
+  const int* lengths;  // [B], may be null (all S)
+  int B, S, H, Hkv, hd, window, sinks;
+  float scale;
+  int* status;
+};
+int window_attention_fwd(const WindowAttnArgs& a, cudaStream_t stream);
+
+struct WindowAttnBwdArgs {
+  WindowAttnArgs f;  // o and lse as the forward left them
+  const __nv_bfloat16* dout;  // [B * S][ldo]
+  int64_t ldo;
+  float* Dbuf;          // [B][H][S] scratch
+  __nv_bfloat16* dqkv;  // [B * S][(H + 2 Hkv) hd]
+};
+int window_attention_bwd(const WindowAttnBwdArgs& a, cudaStream_t stream);
+
 }  // namespace ewb

@@ -1,0 +1,425 @@
+// Attention of one new token a sequence over a ring of keys and values, and
+// filling that ring from a prompt.
+//
+// The ring holds `cap` slots of [k (Hkv heads) | v (Hkv heads)] rows a
+// sequence. The first `sinks` positions keep their slots for good; position
+// p >= sinks sits in slot sinks + (p - sinks) mod (cap - sinks). A token at
+// position p sees the sinks and the positions p - w + 1 .. p, with w the window
+// or, where that is less, the cap - sinks positions that the ring still holds.
+// A cache that never fills is the same rule without a wrap.
+//
+// Bound by memory: every visible row is read once (4 Hkv hd bytes). One cluster
+// of 1 to 8 CTAs serves one (sequence, kv head, up to 16 of its query heads);
+// its warps take groups of 16 visible rows in turn, straight from global memory
+// into mma fragments, with a softmax of their own each (running maximum and sum in
+// fp32); warps join in shared memory, CTAs through distributed shared memory,
+// both in a fixed order. The contraction order of q.k is free, so a lane's 16
+// bytes of a key row serve two k-steps of m16n8k16 as they lie, and a value
+// row's 16 bytes serve eight column tiles; neither needs a transpose. The
+// legacy mma is enough here: at 16 query rows it runs at a few per cent.
+// p is split into two bf16 terms (p = hi + lo), so the second product keeps
+// about 16 bits of each weight; the tensor pipe idles anyway.
+#include "common.cuh"
+#include "kernels.h"
+
+#include <algorithm>
+
+namespace ewb {
+namespace {
+
+constexpr int kStWarps = 8;
+constexpr int kStThreads = kStWarps * 32;
+constexpr int kStHeads = 16;  // query heads of one CTA (the m of the mma)
+constexpr int kStKeys = 16;   // rows of one group
+constexpr float kLog2eSt = 1.4426950408889634f;
+
+__device__ __forceinline__ float ex2_st(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint4 ld16_st(const __nv_bfloat16* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 ld8_st(const __nv_bfloat16* p) {
+  uint2 v;
+  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint32_t ld4_st(const __nv_bfloat16* p) {
+  uint32_t v;
+  asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+
+__device__ __forceinline__ void mma_st(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                       uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ float peer_f32_st(uint32_t a) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+
+// The two bf16 terms of a pair of weights.
+__device__ __forceinline__ void split2(float p0, float p1, uint32_t& hi, uint32_t& lo) {
+  hi = pack_bf16x2(p0, p1);
+  lo = pack_bf16x2(p0 - __uint_as_float(hi << 16), p1 - __uint_as_float(hi & 0xffff0000u));
+}
+
+// The columns of one key row that a lane (q = lane % 4) multiplies: HD / 32
+// vectors of 8 at 32 c + 8 q, then, for HD % 32 == 16, 4 at HD - 16 + 4 q.
+template <int HD>
+struct KeyFrag {
+  static constexpr int kFull = HD / 32;
+  static constexpr bool kHalf = HD % 32 != 0;
+  uint4 w[kFull > 0 ? kFull : 1];
+  uint2 t;
+  __device__ __forceinline__ void load(const __nv_bfloat16* row, int q) {
+#pragma unroll
+    for (int c = 0; c < kFull; ++c) w[c] = ld16_st(row + 32 * c + 8 * q);
+    if constexpr (kHalf) t = ld8_st(row + HD - 16 + 4 * q);
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int c = 0; c < kFull; ++c) w[c] = make_uint4(0, 0, 0, 0);
+    t = make_uint2(0, 0);
+  }
+};
+
+// The columns of one value row that a lane (g = lane / 4) carries into column
+// tiles: HD / 64 vectors of 8 at 64 h + 8 g, then HD % 64 / 8 columns of the rest.
+template <int HD>
+struct ValFrag {
+  static constexpr int kFull = HD / 64;
+  static constexpr int kRest = HD % 64 / 8;  // 0, 2 or 4 columns a lane
+  static constexpr int kWords = 4 * kFull + kRest / 2;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const __nv_bfloat16* row, int g) {
+#pragma unroll
+    for (int h = 0; h < kFull; ++h) {
+      const uint4 v = ld16_st(row + 64 * h + 8 * g);
+      w[4 * h] = v.x;
+      w[4 * h + 1] = v.y;
+      w[4 * h + 2] = v.z;
+      w[4 * h + 3] = v.w;
+    }
+    if constexpr (kRest == 4) {
+      const uint2 v = ld8_st(row + 64 * kFull + 4 * g);
+      w[4 * kFull] = v.x;
+      w[4 * kFull + 1] = v.y;
+    }
+    if constexpr (kRest == 2) w[4 * kFull] = ld4_st(row + 64 * kFull + 2 * g);
+  }
+  // The column of the row that tile t, mma column n holds.
+  __device__ static __forceinline__ int column(int t, int n) {
+    return t < 8 * kFull ? 64 * (t / 8) + 8 * n + t % 8
+                         : 64 * kFull + kRest * n + (t - 8 * kFull);
+  }
+};
+
+template <int HD>
+__global__ void __launch_bounds__(kStThreads, 1)
+    window_step_kernel(const __nv_bfloat16* __restrict__ qkv, int64_t ldq, __nv_bfloat16* cache,
+                       int64_t stride_b, int64_t stride_s, const int64_t* __restrict__ pos,
+                       __nv_bfloat16* __restrict__ o, int H, int Hkv, int htiles, int cluster,
+                       int window, int sinks, int cap, float scale_log2) {
+  extern __shared__ float st_smem[];  // [warps][rows][HD] partial outputs
+  __shared__ float sh_m[kStWarps][kStHeads], sh_l[kStWarps][kStHeads];
+  __shared__ float cta_m[kStHeads], cta_l[kStHeads];
+  constexpr int kTiles = HD / 8;
+
+  const int part = blockIdx.x % cluster;
+  int64_t rest = blockIdx.x / cluster;
+  const int ht = static_cast<int>(rest % htiles);
+  rest /= htiles;
+  const int hk = static_cast<int>(rest % Hkv);
+  const int64_t b = rest / Hkv;
+  const int rep = H / Hkv;
+  const int h0 = hk * rep + ht * kStHeads;       // first query head of this cluster
+  const int rows = min(kStHeads, rep - ht * kStHeads);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  const int64_t p = pos[b];
+  __nv_bfloat16* orow = o + (b * H + h0) * HD;
+  if (p < 0) {  // idle: the same for the whole cluster
+    if (part == 0)
+      for (int i = threadIdx.x; i < rows * HD; i += kStThreads) orow[i] = __float2bfloat16_rn(0.f);
+    return;
+  }
+  const int turn = cap - sinks;
+  const int64_t lo = p + 1 - min(window, turn);
+  const int ns = p < sinks ? static_cast<int>(p) + 1 : sinks;  // visible sinks
+  const int64_t first = lo > sinks ? lo : sinks;               // then first .. p
+  const int n = ns + (p >= first ? static_cast<int>(p + 1 - first) : 0);
+  const int f0 = static_cast<int>((first - sinks) % turn);
+
+  const __nv_bfloat16* newk = qkv + b * ldq + static_cast<int64_t>(H) * HD + hk * HD;
+  const int64_t kv_off = static_cast<int64_t>(Hkv) * HD;  // from a head's k to its v
+  __nv_bfloat16* base = cache + b * stride_b + hk * HD;
+  // Row i of the visible list (i < n); the last one is the new token itself.
+  auto row = [&](int i) -> const __nv_bfloat16* {
+    if (i >= n - 1) return newk;
+    int s = i;
+    if (i >= ns) {
+      s = f0 + (i - ns);
+      s = sinks + (s >= turn ? s - turn : s);
+    }
+    return base + s * stride_s;
+  };
+
+  KeyFrag<HD> qa, qb;  // query heads g and g + 8
+  qa.zero();
+  qb.zero();
+  const __nv_bfloat16* qrow = qkv + b * ldq + static_cast<int64_t>(h0) * HD;
+  if (g < rows) qa.load(qrow + g * HD, q);
+  if (g + 8 < rows) qb.load(qrow + (g + 8) * HD, q);
+
+  float acc[kTiles][4];
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
+  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+
+  const int groups = (n + kStKeys - 1) / kStKeys, all_warps = cluster * kStWarps;
+  for (int G = part * kStWarps + warp; G < groups; G += all_warps) {
+    const int i0 = G * kStKeys;
+    KeyFrag<HD> k0, k1;
+    ValFrag<HD> v[4];
+    k0.load(row(min(i0 + g, n - 1)), q);
+    k1.load(row(min(i0 + 8 + g, n - 1)), q);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      v[e].load(row(min(i0 + 2 * q + (e & 1) + 8 * (e >> 1), n - 1)) + kv_off, g);
+    float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < KeyFrag<HD>::kFull; ++c) {
+      mma_st(s0, qa.w[c].x, qb.w[c].x, qa.w[c].y, qb.w[c].y, k0.w[c].x, k0.w[c].y);
+      mma_st(s1, qa.w[c].x, qb.w[c].x, qa.w[c].y, qb.w[c].y, k1.w[c].x, k1.w[c].y);
+      mma_st(s0, qa.w[c].z, qb.w[c].z, qa.w[c].w, qb.w[c].w, k0.w[c].z, k0.w[c].w);
+      mma_st(s1, qa.w[c].z, qb.w[c].z, qa.w[c].w, qb.w[c].w, k1.w[c].z, k1.w[c].w);
+    }
+    if constexpr (KeyFrag<HD>::kHalf) {
+      mma_st(s0, qa.t.x, qb.t.x, qa.t.y, qb.t.y, k0.t.x, k0.t.y);
+      mma_st(s1, qa.t.x, qb.t.x, qa.t.y, qb.t.y, k1.t.x, k1.t.y);
+    }
+    // this lane: rows g (x0) and g + 8 (x1), keys 2q, 2q + 1, 2q + 8, 2q + 9
+    float x0[4] = {s0[0], s0[1], s1[0], s1[1]}, x1[4] = {s0[2], s0[3], s1[2], s1[3]};
+    float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool ok = i0 + 2 * q + (e & 1) + 8 * (e >> 1) < n;
+      x0[e] = ok ? x0[e] * scale_log2 : -INFINITY;
+      x1[e] = ok ? x1[e] * scale_log2 : -INFINITY;
+      mx0 = fmaxf(mx0, x0[e]);
+      mx1 = fmaxf(mx1, x1[e]);
+    }
+#pragma unroll
+    for (int d = 1; d < 4; d <<= 1) {
+      mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, d));
+      mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, d));
+    }
+    // a group has a visible row, so the maxima are finite (or the data is not)
+    const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
+    const float a0 = m0 == -INFINITY ? 0.f : ex2_st(m0 - n0);
+    const float a1 = m1 == -INFINITY ? 0.f : ex2_st(m1 - n1);
+    m0 = n0;
+    m1 = n1;
+    float r0 = 0.f, r1 = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x0[e] = ex2_st(x0[e] - n0);
+      x1[e] = ex2_st(x1[e] - n1);
+      r0 += x0[e];
+      r1 += x1[e];
+    }
+    l0 = l0 * a0 + r0;
+    l1 = l1 * a1 + r1;
+    uint32_t ph[4], pl[4];
+    split2(x0[0], x0[1], ph[0], pl[0]);
+    split2(x1[0], x1[1], ph[1], pl[1]);
+    split2(x0[2], x0[3], ph[2], pl[2]);
+    split2(x1[2], x1[3], ph[3], pl[3]);
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+      acc[t][0] *= a0;
+      acc[t][1] *= a0;
+      acc[t][2] *= a1;
+      acc[t][3] *= a1;
+      const int wi = t / 2;
+      const uint32_t sel = (t & 1) ? 0x7632u : 0x5410u;
+      const uint32_t b0 = __byte_perm(v[0].w[wi], v[1].w[wi], sel);
+      const uint32_t b1 = __byte_perm(v[2].w[wi], v[3].w[wi], sel);
+      mma_st(acc[t], ph[0], ph[1], ph[2], ph[3], b0, b1);
+      mma_st(acc[t], pl[0], pl[1], pl[2], pl[3], b0, b1);
+    }
+  }
+
+  // ---- join the warps of this CTA
+#pragma unroll
+  for (int d = 1; d < 4; d <<= 1) {
+    l0 += __shfl_xor_sync(0xffffffffu, l0, d);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, d);
+  }
+  if (q == 0) {
+    sh_m[warp][g] = m0;
+    sh_m[warp][g + 8] = m1;
+    sh_l[warp][g] = l0;
+    sh_l[warp][g + 8] = l1;
+  }
+  float* mine = st_smem + warp * rows * HD;
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int col = ValFrag<HD>::column(t, 2 * q + e);
+      if (g < rows) mine[g * HD + col] = acc[t][e];
+      if (g + 8 < rows) mine[(g + 8) * HD + col] = acc[t][2 + e];
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * HD; i += kStThreads) {
+    const int r = i / HD;
+    float M = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kStWarps; ++k) M = fmaxf(M, sh_m[k][r]);
+    float L = 0.f, x = 0.f;
+#pragma unroll
+    for (int k = 0; k < kStWarps; ++k) {
+      const float f = sh_m[k][r] == -INFINITY ? 0.f : ex2_st(sh_m[k][r] - M);
+      L += sh_l[k][r] * f;
+      if (f != 0.f) x += st_smem[k * rows * HD + i] * f;
+    }
+    st_smem[i] = x;
+    if (i % HD == 0) {
+      cta_m[r] = M;
+      cta_l[r] = L;
+    }
+  }
+  // ---- join the CTAs of the cluster; each writes a share of the output
+  if (cluster > 1) {
+    cluster_sync_all();
+    for (int i = part * kStThreads + threadIdx.x; i < rows * HD; i += cluster * kStThreads) {
+      const int r = i / HD;
+      float M = -INFINITY;
+      for (int k = 0; k < cluster; ++k) M = fmaxf(M, peer_f32_st(peer_smem(smem_u32(&cta_m[r]), k)));
+      float L = 0.f, x = 0.f;
+      for (int k = 0; k < cluster; ++k) {
+        const float mk = peer_f32_st(peer_smem(smem_u32(&cta_m[r]), k));
+        const float f = mk == -INFINITY ? 0.f : ex2_st(mk - M);
+        L += peer_f32_st(peer_smem(smem_u32(&cta_l[r]), k)) * f;
+        x += peer_f32_st(peer_smem(smem_u32(&st_smem[i]), k)) * f;
+      }
+      orow[i] = __float2bfloat16_rn(x / L);
+    }
+    cluster_sync_all();  // nobody leaves while its shared memory is read
+  } else {
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * HD; i += kStThreads)
+      orow[i] = __float2bfloat16_rn(st_smem[i] / cta_l[i / HD]);
+  }
+  // ---- the new row enters the ring; its slot is not among those read here:
+  // what sat in it lies cap - sinks positions back, outside the window
+  if (part == 0 && ht == 0 && warp == 0) {
+    const int64_t s = p < sinks ? p : sinks + (p - sinks) % turn;
+    __nv_bfloat16* dst = base + s * stride_s;
+    for (int c = lane; c < 2 * (HD / 8); c += 32) {
+      const int64_t off = c < HD / 8 ? 8 * c : kv_off + 8 * (c - HD / 8);
+      *reinterpret_cast<uint4*>(dst + off) = *reinterpret_cast<const uint4*>(newk + off);
+    }
+  }
+}
+
+template <int HD>
+int launch_step(const WindowStepArgs& a, cudaStream_t stream) {
+  const int rep = a.H / a.Hkv, htiles = (rep + kStHeads - 1) / kStHeads;
+  const int64_t units = a.B * a.Hkv * htiles;
+  const int64_t visible = std::min<int64_t>(a.cap, static_cast<int64_t>(std::min(a.window, a.cap - a.sinks)) + a.sinks);
+  // CTAs a unit: while the units leave SMs idle and every warp keeps a group
+  int cluster = 1;
+  while (cluster < 8 && units * cluster * 2 <= 2 * 148 && visible >= static_cast<int64_t>(cluster) * 2 * kStWarps * kStKeys)
+    cluster *= 2;
+  if (units * cluster > 0x7fffffffll) return 1;
+  const size_t smem = static_cast<size_t>(kStWarps) * std::min(rep, kStHeads) * HD * sizeof(float);
+  static bool attr = false;
+  if (!attr) {
+    if (cudaFuncSetAttribute(window_step_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kStWarps * kStHeads * HD * static_cast<int>(sizeof(float))) != cudaSuccess)
+      return 2;
+    attr = true;
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(units * cluster));
+  cfg.blockDim = dim3(kStThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, window_step_kernel<HD>, a.qkv, a.ldq, a.cache, a.stride_b,
+                            a.stride_s, a.pos, a.o, a.H, a.Hkv, htiles, cluster, a.window, a.sinks,
+                            a.cap, a.scale * kLog2eSt) == cudaSuccess
+             ? 0
+             : 2;
+}
+
+// ---------------------------------------------------------------- prompt
+// Copies the k | v columns of prompt rows into the ring: of a sequence of n
+// positions, the sinks and the last cap - sinks.
+__global__ void __launch_bounds__(256)
+    window_fill_kernel(const __nv_bfloat16* __restrict__ qkv, int64_t ldq, int kv_col,
+                       __nv_bfloat16* __restrict__ cache, int64_t stride_b, int64_t stride_s,
+                       const int* __restrict__ lengths, int64_t rows, int S, int vecs, int sinks,
+                       int cap) {
+  const int turn = cap - sinks;
+  for (int64_t t = blockIdx.x; t < rows; t += gridDim.x) {
+    const int64_t b = t / S;
+    const int s = static_cast<int>(t - b * S);
+    const int n = lengths != nullptr ? min(max(lengths[b], 0), S) : S;
+    if (s >= n || (s >= sinks && s < n - turn)) continue;
+    const int slot = s < sinks ? s : sinks + (s - sinks) % turn;
+    const uint4* src = reinterpret_cast<const uint4*>(qkv + t * ldq + kv_col);
+    uint4* dst = reinterpret_cast<uint4*>(cache + b * stride_b + slot * stride_s);
+    for (int v = threadIdx.x; v < vecs; v += 256) dst[v] = src[v];
+  }
+}
+
+}  // namespace
+
+int window_step(const WindowStepArgs& a, cudaStream_t stream) {
+  if (a.B < 0 || a.H < 1 || a.Hkv < 1 || a.H % a.Hkv || a.window < 1 || a.sinks < 0 || a.cap <= a.sinks)
+    return 1;
+  if (a.B == 0) return 0;
+  switch (a.hd) {
+    case 64: return launch_step<64>(a, stream);
+    case 80: return launch_step<80>(a, stream);
+    case 96: return launch_step<96>(a, stream);
+    case 128: return launch_step<128>(a, stream);
+    default: return 1;
+  }
+}
+
+int window_fill(const WindowFillArgs& a, cudaStream_t stream) {
+  if (a.B < 0 || a.S < 0 || a.sinks < 0 || a.cap <= a.sinks || a.width % 8) return 1;
+  const int64_t rows = a.B * a.S;
+  if (rows == 0) return 0;
+  window_fill_kernel<<<static_cast<unsigned>(std::min<int64_t>(rows, 148 * 32)), 256, 0, stream>>>(
+      a.qkv, a.ldq, a.kv_col, a.cache, a.stride_b, a.stride_s, a.lengths, rows, a.S, a.width / 8,
+      a.sinks, a.cap);
+  return cudaGetLastError() == cudaSuccess ? 0 : 2;
+}
+
+}  // namespace ewb

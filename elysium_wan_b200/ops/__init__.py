@@ -21,6 +21,10 @@ import torch
 import torch.nn.functional as F
 
 from ._ext import ext, launch_count  # noqa: F401
+from .dropout import dropout_add, dropout_bwd, dropout_words  # noqa: F401
+from .logprobs import TokenLogprobs, token_logprobs, token_logprobs_bwd  # noqa: F401
+from .window import (ring_slot, window_attention_bwd, window_attention_fwd,  # noqa: F401
+                     window_attention_step, window_cache_fill)
 
 E4M3 = torch.float8_e4m3fn
 E5M2 = torch.float8_e5m2

@@ -1,0 +1,99 @@
+"""Log probabilities of given tokens, entropy and top alternatives of logit rows."""
+
+from __future__ import annotations
+
+import math
+from typing import NamedTuple
+
+import torch
+
+from ._ext import ext
+
+TOP_MAX = 32
+
+
+class TokenLogprobs(NamedTuple):
+    """Per row, natural logarithms in fp32: logp [T] (None without targets),
+    entropy [T], lse [T] (log sum exp), top_logp [T, top] and top_ids [T, top]
+    int64 (None for top 0)."""
+
+    logp: torch.Tensor | None
+    entropy: torch.Tensor
+    lse: torch.Tensor
+    top_logp: torch.Tensor | None
+    top_ids: torch.Tensor | None
+
+
+def token_logprobs(logits, V: int, targets=None, *, top: int = 0) -> TokenLogprobs:
+    """Statistics of the first V columns of bf16 or fp32 logits [T, ld].
+
+    targets: int64 [T]; a negative one says that the row has no given token
+    (logp 0), one at or past V gives NaN (and on the GPU an entry in the status
+    record). top: how many of the most probable tokens to return, at most 32;
+    of equal logits the lowest index comes first.
+
+    A logit of -inf has probability 0. A row of nothing else has lse -inf,
+    entropy 0 and log probabilities -inf. A row with a NaN or +inf has NaN
+    statistics, and -1 for its alternatives.
+    """
+    if logits.is_cuda:
+        return TokenLogprobs(*ext().token_logprobs(logits, V, targets, top))
+    if logits.dim() != 2 or not 1 <= V <= logits.shape[1]:
+        raise ValueError("logits must be [T, ld] with V columns")
+    if not 0 <= top <= min(TOP_MAX, V):
+        raise ValueError(f"top must be in [0, {TOP_MAX}] and no more than V")
+    if targets is not None and targets.numel() != logits.shape[0]:
+        raise ValueError("targets must have one entry for each row")
+    x = logits[:, :V].float()
+    nan = torch.isnan(x).any(1) | (x == math.inf).any(1)
+    m = x.amax(1, keepdim=True)
+    m = torch.where(m == -math.inf, 0.0, m)
+    lns = torch.log(torch.exp(x - m).sum(1, keepdim=True))
+    lse = (m + lns)[:, 0].masked_fill(nan, math.nan)
+    lns = torch.where(lns == -math.inf, 0.0, lns)
+    lp = (x - m) - lns
+    p = torch.exp(lp)
+    entropy = -torch.where(p > 0, p * lp, 0.0).sum(1).masked_fill(nan, math.nan)
+    logp = top_logp = top_ids = None
+    if targets is not None:
+        t = targets.reshape(-1)
+        logp = lp.gather(1, t.clamp(0, V - 1)[:, None])[:, 0]
+        logp = torch.where(t < 0, 0.0, torch.where(t >= V, math.nan, logp))
+    if top:
+        v, ids = torch.sort(x, dim=1, descending=True, stable=True)
+        top_logp = ((v[:, :top] - m) - lns).masked_fill(nan[:, None], math.nan)
+        top_ids = ids[:, :top].masked_fill(nan[:, None], -1)
+    return TokenLogprobs(logp, entropy, lse, top_logp, top_ids)
+
+
+def token_logprobs_bwd(logits, V: int, targets, lse, entropy, g_logp=None, g_entropy=None, *,
+                       ld_grad: int | None = None, out_dtype=None):
+    """Gradient of sum_t g_logp[t] logp[t] + g_entropy[t] entropy[t] with
+    respect to the logits: [T, ld_grad], columns from V on 0.
+
+    lse and entropy come from token_logprobs on the same logits; probabilities
+    are e^(x - lse), so their relative error is that of the fp32 lse, |lse| /
+    2**24. ld_grad is
+    V rounded up to 8 unless given (the row length that the GEMMs read through
+    TMA); out_dtype is bf16 unless given (fp32 on the host path).
+    """
+    if ld_grad is None:
+        ld_grad = (V + 7) // 8 * 8
+    if logits.is_cuda:
+        return ext().token_logprobs_bwd(logits, V, targets, lse, entropy, g_logp, g_entropy,
+                                        ld_grad, out_dtype or torch.bfloat16)
+    if ld_grad < V:
+        raise ValueError("ld_grad must be at least V")
+    x = logits[:, :V].float()
+    u = x - torch.where(lse == -math.inf, math.inf, lse)[:, None]
+    p = torch.exp(u)
+    zero = torch.zeros_like(lse)
+    t = targets.reshape(-1) if targets is not None else torch.full(lse.shape, -1)
+    given = (t >= 0) & (t < V)
+    gl = torch.where(given, g_logp if g_logp is not None else zero, 0.0)
+    ge = (g_entropy if g_entropy is not None else zero)[:, None]
+    d = -torch.where(p == 0, 0.0, p * (gl[:, None] + ge * (u + entropy[:, None])))
+    d.scatter_add_(1, t.clamp(0, V - 1)[:, None], gl[:, None])
+    out = torch.zeros((x.shape[0], ld_grad), dtype=out_dtype or torch.float32)
+    out[:, :V] = d
+    return out

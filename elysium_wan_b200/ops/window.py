@@ -1,0 +1,162 @@
+"""Attention in a sliding window with sinks: training over packed rows, and one
+new token a sequence over a ring of keys and values.
+
+Query i sees key j <= i when i - j < window or j < sinks (the first tokens stay
+visible), and when both lie below the sequence's length. Heads may be grouped
+(Hkv < H): query head h reads kv head h // (H // Hkv).
+
+Tensors are those of the full attention: rows of q (H heads) | k (Hkv) | v
+(Hkv), hd columns a head. The GPU kernels take hd 64, 80, 96 and 128, any
+number of rows, and rows that are strided as long as they are 16-byte aligned.
+What lies in rows at or past a sequence's length is never used, NaN included.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from ._ext import ext
+
+_LOG2E = 1.0 / math.log(2.0)
+
+
+def _check(qkv, rows, H, hd, Hkv, window, sinks):
+    if H < 1 or Hkv < 1 or H % Hkv:
+        raise ValueError("H must be a multiple of Hkv")
+    if window < 1 or sinks < 0:
+        raise ValueError("window must be at least 1 and sinks at least 0")
+    if qkv.dim() != 2 or qkv.shape[0] != rows or qkv.shape[1] != (H + 2 * Hkv) * hd:
+        raise ValueError(f"qkv must be [{rows}, {(H + 2 * Hkv) * hd}], got {list(qkv.shape)}")
+
+
+def ring_slot(pos, sinks: int, slots: int):
+    """The slot of position pos in a ring of `slots` rows (ints or tensors)."""
+    turn = slots - sinks
+    if isinstance(pos, torch.Tensor):
+        return torch.where(pos < sinks, pos, sinks + (pos - sinks) % turn)
+    return pos if pos < sinks else sinks + (pos - sinks) % turn
+
+
+def _visible(S, window, sinks, lengths):
+    i, j = torch.arange(S)[:, None], torch.arange(S)[None, :]
+    m = (j <= i) & ((i - j < window) | (j < sinks))
+    if lengths is None:
+        return m[None, None]
+    n = lengths.view(-1, 1, 1, 1)
+    return m & (i < n) & (j < n)
+
+
+def _heads(qkv, B, S, H, hd, Hkv, lengths):
+    """q, k, v [B, H, S, hd] in fp32, kv heads repeated, rows past a length 0."""
+    x = qkv.float().view(B, S, H + 2 * Hkv, hd).transpose(1, 2)
+    if lengths is not None:
+        x = torch.where(torch.arange(S)[:, None] < lengths.view(-1, 1, 1, 1), x, 0.0)
+    rep = H // Hkv
+    return (x[:, :H], x[:, H:H + Hkv].repeat_interleave(rep, 1),
+            x[:, H + Hkv:].repeat_interleave(rep, 1))
+
+
+def _probs(q, k, hd, seen):
+    """(softmax, base-2 log-sum-exp) of the visible scores; an empty row is 0, -inf."""
+    x = (q @ k.mT / math.sqrt(hd)).masked_fill(~seen, -math.inf)
+    lse = torch.logsumexp(x, -1)
+    return torch.exp(x - torch.where(lse == -math.inf, 0.0, lse)[..., None]), lse * _LOG2E
+
+
+def window_attention_fwd(qkv, B, S, H, hd, Hkv=None, *, window, sinks=0, lengths=None):
+    """(o [B*S, H*hd], lse [B, H, S] base 2) of attention in a sliding window.
+
+    lengths: int32 [B] on qkv's device, None for full sequences; a value
+    outside [0, S] counts as the nearer bound. Rows past it: o 0, lse -inf.
+    """
+    Hkv = Hkv or H
+    if qkv.is_cuda:
+        return ext().window_attention_fwd(qkv, B, S, H, hd, Hkv, window, sinks, lengths,
+                                          1.0 / math.sqrt(hd))
+    _check(qkv, B * S, H, hd, Hkv, window, sinks)
+    q, k, v = _heads(qkv, B, S, H, hd, Hkv, lengths)
+    p, lse = _probs(q, k, hd, _visible(S, window, sinks, lengths))
+    return (p @ v).transpose(1, 2).reshape(B * S, H * hd), lse
+
+
+def window_attention_bwd(qkv, o, dout, lse, B, S, H, hd, Hkv=None, *, window, sinks=0,
+                         lengths=None):
+    """Gradient of qkv (its layout, dense); o and lse as the forward gave them.
+    A kv head's gradient sums its group's query heads in head order; rows past
+    a sequence's length get 0."""
+    Hkv = Hkv or H
+    if qkv.is_cuda:
+        return ext().window_attention_bwd(qkv, o, dout, lse, B, S, H, hd, Hkv, window, sinks,
+                                          lengths, 1.0 / math.sqrt(hd))
+    _check(qkv, B * S, H, hd, Hkv, window, sinks)
+    q, k, v = _heads(qkv, B, S, H, hd, Hkv, lengths)
+    p, _ = _probs(q, k, hd, _visible(S, window, sinks, lengths))
+    do = dout.float().view(B, S, H, hd).transpose(1, 2)
+    if lengths is not None:
+        do = torch.where(torch.arange(S)[:, None] < lengths.view(-1, 1, 1, 1), do, 0.0)
+    dp = do @ v.mT
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True)) / math.sqrt(hd)
+    group = lambda t: t.view(B, Hkv, H // Hkv, S, hd).sum(2)  # noqa: E731
+    d = torch.cat([ds @ k, group(ds.mT @ q), group(p.mT @ do)], 1)
+    return d.transpose(1, 2).reshape(B * S, -1)
+
+
+def window_attention_step(qkv, cache, pos, H, hd, Hkv=None, *, window, sinks=0):
+    """One new token a sequence: o [B, H*hd] from rows qkv [B, (H + 2 Hkv) hd].
+
+    cache [B, slots, 2 * Hkv * hd] (bf16 on the GPU) is a ring of k | v rows:
+    the first `sinks` positions keep their slots, position p >= sinks sits in
+    slot sinks + (p - sinks) % (slots - sinks), so slots = sinks + window serves
+    an answer of any length, and a cache that never fills does not wrap. The
+    new rows' k | v enter the cache here. A window wider than the ring sees
+    what the ring holds. pos: int64 [B], the new tokens' positions (the number
+    of tokens before them); a negative one marks an idle sequence, whose o is 0
+    and whose cache stays. Positional rotation of q and k is the caller's, as
+    for the training rows.
+    """
+    Hkv = Hkv or H
+    B = qkv.shape[0]
+    if qkv.is_cuda:
+        return ext().window_step(qkv, cache, pos, H, hd, Hkv, window, sinks, 1.0 / math.sqrt(hd))
+    _check(qkv, B, H, hd, Hkv, window, sinks)
+    _check_ring(cache, B, hd, Hkv, sinks)
+    slots = cache.shape[1]
+    o = torch.zeros((B, H * hd))
+    for b, p in enumerate(pos.tolist()):
+        if p < 0:
+            continue
+        cache[b, ring_slot(p, sinks, slots)] = qkv[b, H * hd:].to(cache.dtype)
+        first = max(sinks, p + 1 - min(window, slots - sinks))
+        at = torch.cat([torch.arange(min(sinks, p + 1)), torch.arange(first, max(first, p + 1))])
+        kv = cache[b, ring_slot(at, sinks, slots)].float().view(-1, 2, Hkv, hd)
+        q = qkv[b, :H * hd].float().view(Hkv, H // Hkv, hd)
+        w = torch.softmax(q @ kv[:, 0].permute(1, 2, 0) / math.sqrt(hd), -1)
+        o[b] = (w @ kv[:, 1].transpose(0, 1)).reshape(-1)
+    return o
+
+
+def _check_ring(cache, B, hd, Hkv, sinks):
+    if cache.dim() != 3 or cache.shape[0] != B or cache.shape[2] != 2 * Hkv * hd:
+        raise ValueError("cache must be [B, slots, 2 * Hkv * hd]")
+    if cache.shape[1] <= sinks:
+        raise ValueError("cache must have more slots than sinks")
+
+
+def window_cache_fill(qkv, cache, B, S, H, hd, Hkv=None, *, sinks=0, lengths=None):
+    """Put a prompt's k | v rows into the ring (the sinks and what fits of the
+    latest positions); the next token's position is the prompt's length."""
+    Hkv = Hkv or H
+    if qkv.is_cuda:
+        ext().window_fill(qkv, cache, B, S, H, hd, Hkv, sinks, lengths)
+        return
+    _check(qkv, B * S, H, hd, Hkv, 1, sinks)
+    _check_ring(cache, B, hd, Hkv, sinks)
+    slots = cache.shape[1]
+    kv = qkv.view(B, S, -1)[:, :, H * hd:]
+    for b in range(B):
+        n = S if lengths is None else min(max(int(lengths[b]), 0), S)
+        p = torch.arange(n)
+        p = p[(p < sinks) | (p >= n - (slots - sinks))]
+        cache[b, ring_slot(p, sinks, slots)] = kv[b, p].to(cache.dtype)

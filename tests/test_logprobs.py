@@ -1,0 +1,259 @@
+"""Log probabilities of given tokens, entropy, alternatives and the gradient.
+
+Would fail if: a row's sums lost terms at an odd start or a ragged end, ties
+went to another index than the lowest, a masked vocabulary or an empty row gave
+NaN, many rows and few rows (one CTA or a cluster a row) disagreed, the
+alternatives depended on the order of arrival, or the gradient left its formula.
+"""
+
+import math
+
+import pytest
+import torch
+
+from elysium_wan_b200 import ops
+
+NAN, INF = math.nan, math.inf
+
+
+def plain64(x, V, t, top):
+    # from the row's maximum: at the type's lowest value even 64 bits drop ln V
+    x = x[:, :V].double()
+    m = x.amax(1, keepdim=True)
+    m = torch.where(m == -INF, 0.0, m)
+    lns = torch.logsumexp(x - m, 1, keepdim=True)
+    lse = (m + lns)[:, 0]
+    lp = (x - m) - torch.where(lns == -INF, 0.0, lns)
+    h = torch.special.entr(lp.exp()).sum(1)
+    got = torch.where(t >= 0, lp.gather(1, t.clamp(min=0)[:, None])[:, 0], 0.0)
+    v, ids = torch.sort(x, dim=1, descending=True, stable=True)
+    return got, h, lse, lp.gather(1, ids)[:, :top], ids[:, :top]
+
+
+def grad64(x, V, t, gl, ge):
+    got, h, lse, _, _ = plain64(x, V, t, 0)
+    lp = x[:, :V].double() - torch.where(lse == -INF, INF, lse)[:, None]
+    p = lp.exp()
+    g = torch.where(t >= 0, gl.double(), 0.0)
+    d = -torch.where(p > 0, p * (g[:, None] + ge.double()[:, None] * (lp + h[:, None])), 0.0)
+    return d.scatter_add(1, t.clamp(min=0)[:, None], g[:, None])
+
+
+def logits(T, V, ld, dtype, seed=0, masked=0.0, device="cpu"):
+    g = torch.Generator(device=device)
+    g.manual_seed(seed)
+    x = torch.randn(T, ld, generator=g, device=device)
+    x = (2 * x + 8 * (x > 2.5)).to(dtype)
+    if masked:
+        x = x.masked_fill(torch.rand(T, ld, generator=g, device=device) < masked, -INF)
+    t = torch.randint(-1, V, (T,), generator=g, device=device)
+    return x, t
+
+
+# fp32 statistics: a logit of size 30 is rounded to 2^-24 of it when 2^x's
+# argument is formed, and V terms are summed in trees of about 300 in a row, so
+# absolute errors stay under a few 1e-5 of max(1, |value|); 2e-5 allows that.
+def near(a, b):
+    a, b = a.double(), b.double()
+    same = (a == b) | (torch.isnan(a) & torch.isnan(b))
+    bad = ~same & ~((a - b).abs() <= 2e-5 * b.abs().clamp(min=1.0))
+    assert not bool(bad.any()), (a[bad][:5], b[bad][:5])
+
+
+def check(x, V, t, top):
+    r = ops.token_logprobs(x, V, t, top=top)
+    got, h, lse, tv, ti = plain64(x, V, t, top)
+    near(r.logp, got)
+    near(r.entropy, h)
+    near(r.lse, lse)
+    if top:
+        near(r.top_logp, tv)
+        assert torch.equal(r.top_ids, ti)
+    else:
+        assert r.top_logp is None and r.top_ids is None
+    return r
+
+
+def test_host_path():
+    for masked in (0.0, 0.7):
+        x, t = logits(9, 50, 57, torch.float32, masked=masked)
+        check(x, 50, t, 5)
+    x[3] = -INF
+    r = check(x, 50, t, 50 if 50 <= 32 else 32)
+    assert r.lse[3] == -INF and r.entropy[3] == 0 and r.top_ids[3].tolist() == list(range(32))
+    x[4, 2] = NAN
+    x[5, 2] = INF
+    r = ops.token_logprobs(x, 50, t, top=2)
+    assert torch.isnan(r.entropy[4:6]).all() and (r.top_ids[4:6] == -1).all()
+
+
+def test_host_gradient_against_formula_and_differences():
+    x, t = logits(4, 11, 11, torch.float32)
+    gl, ge = torch.randn(4), torch.randn(4)
+    r = ops.token_logprobs(x, 11, t)
+    d = ops.token_logprobs_bwd(x, 11, t, r.lse, r.entropy, gl, ge)
+    assert d.shape == (4, 16) and bool((d[:, 11:] == 0).all())
+    near(d[:, :11], grad64(x, 11, t, gl, ge))
+    # central differences in 64 bits of the 64-bit plain form: h^2 of the third
+    # derivative, under 1e-6 for h = 1e-3 and unit-size weights
+    for row, col in ((0, 0), (1, 5), (2, 10), (3, 7)):
+        f = []
+        for h in (1e-3, -1e-3):
+            y = x.double().clone()
+            y[row, col] += h
+            got, ent, _, _, _ = plain64(y, 11, t, 0)
+            f.append((gl.double() * got + ge.double() * ent).sum())
+        assert abs((f[0] - f[1]) / 2e-3 - d[row, col]) < 5e-5
+
+
+def test_refusals_host():
+    x, t = logits(3, 8, 8, torch.float32)
+    for kw in (dict(V=9), dict(V=0), dict(V=8, top=9), dict(V=8, top=-1)):
+        with pytest.raises(ValueError):
+            ops.token_logprobs(x, kw.pop("V"), t, **kw)
+    with pytest.raises(ValueError):
+        ops.token_logprobs(x, 8, t[:2])
+    with pytest.raises(ValueError):
+        ops.token_logprobs_bwd(x, 8, t, t.float(), t.float(), ld_grad=7)
+
+
+# ----------------------------------------------------------------------------- GPU
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,V,ld", [(1, 1, 1), (2, 3, 5), (3, 33, 33), (5, 1000, 1003), (1, 128256, 128256),
+                                    (3, 50257, 50257), (40, 8191, 8192), (200, 5003, 5003),
+                                    (2, 200001, 200001)])
+@pytest.mark.parametrize("top", [0, 1, 20, 32])
+def test_gpu_against_plain(cuda, dtype, T, V, ld, top):
+    x, t = logits(T, V, ld, dtype, seed=T + V, device=cuda)
+    check(x, V, t, min(top, V))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [40, 700, 40001])
+def test_gpu_masks_and_empty_rows(cuda, dtype, V):
+    for masked in (0.3, 0.99):
+        x, t = logits(12, V, V + 3, dtype, seed=V, masked=masked, device=cuda)
+        x[0] = -INF
+        x[1, 1:] = -INF
+        x[2, :V - 1] = -INF
+        x[3] = torch.finfo(dtype).min  # a mask of the type's lowest value
+        x[4] = torch.finfo(dtype).min
+        x[4, V // 2] = 0.0
+        r = check(x, V, t, 32)
+        assert r.lse[0] == -INF and r.entropy[0] == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gpu_ties_take_the_lowest_index(cuda, dtype):
+    T, V = 6, 30011
+    x = torch.randint(-3, 4, (T, V), device=cuda).to(dtype)
+    x[0] = 0.0  # one value all over
+    x[1] = torch.where(torch.arange(V, device=cuda) % 2 == 0, 0.0, -0.0).to(dtype)  # 0 and -0 are equal
+    check(x, V, torch.zeros(T, dtype=torch.int64, device=cuda), 32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 2, 400])
+def test_gpu_alternatives_crowded_in_few_threads(cuda, rows):
+    """More logits above the bound than the candidate list holds: the vectors
+    of 32 quads of every round stand out, then all but a few of the row."""
+    for dtype, ve in ((torch.float32, 4), (torch.bfloat16, 8)):
+        V = 512 * ve * 24
+        x = torch.randn(rows, V, device=cuda).to(dtype)
+        thread = (torch.arange(V, device=cuda) // ve) % 512
+        x = torch.where(thread < 128, x + 50, x).contiguous()
+        t = torch.zeros(rows, dtype=torch.int64, device=cuda)
+        check(x, V, t, 32)
+        check(torch.where(thread < 4, x + 50, x).contiguous(), V, t, 20)
+    x = torch.arange(60000, device=cuda, dtype=torch.float32).expand(rows, 60000) / 1000
+    check(x.contiguous(), 60000, t, 32)
+    check(x.flip(1).contiguous(), 60000, t, 32)
+
+
+@pytest.mark.gpu
+def test_gpu_rows_do_not_depend_on_how_many_there_are(cuda):
+    """One CTA a row (many rows) and a cluster a row (few) agree: ids equal,
+    statistics within the bound, and each is bitwise the same from call to call."""
+    x, t = logits(400, 60013, 60013, torch.float32, device=cuda)
+    many = ops.token_logprobs(x, 60013, t, top=32)
+    again = ops.token_logprobs(x, 60013, t, top=32)
+    for a, b in zip(many, again):
+        assert torch.equal(a, b)
+    for r in (0, 17, 399):
+        one = ops.token_logprobs(x[r:r + 1], 60013, t[r:r + 1], top=32)
+        assert torch.equal(one.top_ids[0], many.top_ids[r])
+        near(one.lse, many.lse[r:r + 1])
+        near(one.entropy, many.entropy[r:r + 1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [37, 20000])
+def test_gpu_nan_inf_and_bad_targets(cuda, dtype, V):
+    x, t = logits(5, V, V, dtype, device=cuda)
+    x[0, 3] = NAN
+    x[1, V - 1] = INF
+    x[2] = NAN
+    t[3], t[4] = V, -7
+    ops.ext().status_read_clear()
+    r = ops.token_logprobs(x, V, t, top=3)
+    assert ops.ext().status_record()[2:] == [3, V]  # the row and the target that it names
+    assert ops.ext().status_read_clear() == 6
+    for row in (0, 1, 2):
+        assert torch.isnan(r.entropy[row]) and torch.isnan(r.lse[row])
+        assert torch.isnan(r.top_logp[row]).all() and (r.top_ids[row] == -1).all()
+    assert torch.isnan(r.logp[3]) and r.logp[4] == 0
+    assert torch.isfinite(r.entropy[3:]).all()
+    d = ops.token_logprobs_bwd(x, V, t, r.lse, r.entropy, torch.ones(5, device=cuda), None)
+    assert torch.isfinite(d[3:]).all() and torch.isnan(d[0, :V].float()).any()
+    assert bool((d[3:] == 0).all())  # no given token, no entropy weight
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,out", [(torch.float32, torch.float32), (torch.float32, torch.bfloat16),
+                                       (torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32)])
+@pytest.mark.parametrize("T,V,ld,ldg", [(1, 5, 5, 8), (7, 1000, 1008, 1000), (33, 5003, 5003, 5003),
+                                        (4, 5003, 5008, 5008), (2, 70000, 70001, 70016)])
+def test_gpu_gradient(cuda, dtype, out, T, V, ld, ldg):
+    x, t = logits(T, V, ld, dtype, seed=V, masked=0.2, device=cuda)
+    t = torch.where(x.gather(1, t.clamp(min=0)[:, None])[:, 0] == -INF, -1, t)
+    if T > 5:
+        x[5] = -INF
+        t[5] = -1
+    gl, ge = torch.randn(T, device=cuda), torch.randn(T, device=cuda)
+    r = ops.token_logprobs(x, V, t)
+    d = ops.token_logprobs_bwd(x, V, t, r.lse, r.entropy, gl, ge, ld_grad=ldg, out_dtype=out)
+    assert d.shape == (T, ldg) and d.dtype == out and bool((d[:, V:] == 0).all())
+    want = grad64(x, V, t, gl, ge)
+    # p carries the fp32 lse's rounding (2^-24 of about 30) and log p + H two
+    # more; then one rounding to the output type
+    unit = 2.0**-8 if out == torch.bfloat16 else 0.0
+    lim = want.abs() * (unit * 1.01 + 1e-5) + 1e-5 * (gl.abs() + ge.abs()).double()[:, None] * want.abs().clamp(max=1.0) + 1e-7
+    assert bool(((d[:, :V].double() - want).abs() <= lim).all())
+    only = ops.token_logprobs_bwd(x, V, t, r.lse, r.entropy, gl, None, ld_grad=ldg, out_dtype=out)
+    want = grad64(x, V, t, gl, torch.zeros_like(ge))
+    assert bool(((only[:, :V].double() - want).abs() <= want.abs() * (unit * 1.01 + 2e-5) + 1e-7).all())
+
+
+@pytest.mark.gpu
+def test_gpu_refusals(cuda):
+    x, t = logits(3, 40, 40, torch.float32, device=cuda)
+    for bad in (dict(V=41), dict(V=0), dict(V=40, top=33), dict(V=10, top=11)):
+        with pytest.raises(RuntimeError):
+            ops.token_logprobs(x, bad.pop("V"), t, **bad)
+    with pytest.raises(RuntimeError, match="targets must be int64"):
+        ops.token_logprobs(x, 40, t.int())
+    with pytest.raises(RuntimeError, match="must be on"):
+        ops.token_logprobs(x, 40, t.cpu())
+    with pytest.raises(RuntimeError, match="bf16 or fp32"):
+        ops.token_logprobs(x.half(), 40, t)
+    r = ops.token_logprobs(x, 40, t)
+    with pytest.raises(RuntimeError, match="ld_grad"):
+        ops.token_logprobs_bwd(x, 40, t, r.lse, r.entropy, ld_grad=39)
+    with pytest.raises(RuntimeError, match="fp32, one for each row"):
+        ops.token_logprobs_bwd(x, 40, t, r.lse[:2], r.entropy)
+    empty = ops.token_logprobs(x[:0], 40, t[:0], top=4)
+    assert empty.top_ids.shape == (0, 4)

@@ -920,6 +920,76 @@ void check_ring(const at::Tensor& cache, const at::Tensor& qkv, int64_t B, int64
               "cache rows must be 16-byte aligned");
 }
 
+ewb::WindowAttnArgs window_args(const at::Tensor& qkv, const c10::optional<at::Tensor>& lengths,
+                                int64_t B, int64_t S, int64_t H, int64_t hd, int64_t Hkv,
+                                int64_t window, int64_t sinks, double scale) {
+  check_window(qkv, H, hd, Hkv, window, sinks);
+  TORCH_CHECK(B >= 0 && S >= 0 && qkv.size(0) == B * S, "qkv must have B * S rows");
+  TORCH_CHECK(B <= 65535 && S <= 65535 * 64, "at most 65535 sequences of 4194240 rows");
+  ewb::WindowAttnArgs f{};
+  f.qkv = reinterpret_cast<const __nv_bfloat16*>(qkv.data_ptr());
+  f.ldq = row_stride(qkv);
+  f.lengths = checked_lengths(lengths, qkv, B);
+  f.B = B;
+  f.S = S;
+  f.H = H;
+  f.Hkv = Hkv;
+  f.hd = hd;
+  f.window = static_cast<int>(std::min<int64_t>(window, 0x7fffffff));
+  f.sinks = static_cast<int>(std::min<int64_t>(sinks, 0x7fffffff));
+  f.scale = static_cast<float>(scale);
+  f.status = status_word(qkv.get_device());
+  return f;
+}
+
+std::vector<at::Tensor> window_attention_fwd(at::Tensor qkv, int64_t B, int64_t S, int64_t H,
+                                             int64_t hd, int64_t Hkv, int64_t window, int64_t sinks,
+                                             c10::optional<at::Tensor> lengths, double scale) {
+  ewb::WindowAttnArgs f = window_args(qkv, lengths, B, S, H, hd, Hkv, window, sinks, scale);
+  c10::cuda::CUDAGuard guard(qkv.device());
+  at::Tensor o = at::empty({B * S, H * hd}, qkv.options());
+  at::Tensor lse = at::empty({B, H, S}, qkv.options().dtype(at::kFloat));
+  f.o = reinterpret_cast<__nv_bfloat16*>(o.data_ptr());
+  f.lse = lse.data_ptr<float>();
+  ok(ewb::window_attention_fwd(f, cur_stream()), "window_attention_fwd");
+  if (B * S > 0) count(1);
+  return {o, lse};
+}
+
+at::Tensor window_attention_bwd(at::Tensor qkv, at::Tensor o, at::Tensor dout, at::Tensor lse,
+                                int64_t B, int64_t S, int64_t H, int64_t hd, int64_t Hkv,
+                                int64_t window, int64_t sinks, c10::optional<at::Tensor> lengths,
+                                double scale) {
+  ewb::WindowAttnBwdArgs a{};
+  a.f = window_args(qkv, lengths, B, S, H, hd, Hkv, window, sinks, scale);
+  check_same_device(o, qkv, "o");
+  check_same_device(dout, qkv, "dout");
+  check_same_device(lse, qkv, "lse");
+  check_inner(dout, "dout");
+  TORCH_CHECK(o.scalar_type() == at::kBFloat16 && o.dim() == 2 && o.size(0) == B * S && o.size(1) == H * hd &&
+                  o.is_contiguous(),
+              "o must be the forward's bf16 [B * S, H * hd]");
+  TORCH_CHECK(dout.scalar_type() == at::kBFloat16 && dout.size(0) == B * S && dout.size(1) == H * hd,
+              "dout must be bf16 [B * S, H * hd]");
+  TORCH_CHECK(aligned16(dout.data_ptr()) && aligned16(o.data_ptr()) && row_stride(dout) % 8 == 0,
+              "dout rows must be 16-byte aligned");
+  TORCH_CHECK(lse.scalar_type() == at::kFloat && lse.is_contiguous() && lse.numel() == B * H * S,
+              "lse must be the forward's fp32 [B, H, S]");
+  c10::cuda::CUDAGuard guard(qkv.device());
+  at::Tensor dqkv = at::empty({B * S, (H + 2 * Hkv) * hd}, qkv.options());
+  if (B * S == 0) return dqkv;
+  at::Tensor ws = at::empty({ewb::window_attention_bwd_ws(a.f)}, qkv.options().dtype(at::kFloat));
+  a.f.o = reinterpret_cast<__nv_bfloat16*>(o.data_ptr());
+  a.f.lse = lse.data_ptr<float>();
+  a.dout = reinterpret_cast<const __nv_bfloat16*>(dout.data_ptr());
+  a.ldo = row_stride(dout);
+  a.ws = ws.data_ptr<float>();
+  a.dqkv = reinterpret_cast<__nv_bfloat16*>(dqkv.data_ptr());
+  ok(ewb::window_attention_bwd(a, cur_stream()), "window_attention_bwd");
+  count(ewb::window_attention_bwd_launches(a.f));
+  return dqkv;
+}
+
 at::Tensor window_step(at::Tensor qkv, at::Tensor cache, at::Tensor pos, int64_t H, int64_t hd,
                        int64_t Hkv, int64_t window, int64_t sinks, double scale) {
   check_window(qkv, H, hd, Hkv, window, sinks);
@@ -998,6 +1068,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("dropout_add", &dropout_add);
   m.def("token_logprobs", &token_logprobs);
   m.def("token_logprobs_bwd", &token_logprobs_bwd);
+  m.def("window_attention_fwd", &window_attention_fwd);
+  m.def("window_attention_bwd", &window_attention_bwd);
   m.def("window_step", &window_step);
   m.def("window_fill", &window_fill);
   m.def("rope", &rope);

@@ -1652,4 +1652,19 @@ bool tma_map_bf16_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_
   return make_map_bf16(map, base, inner, outer, ld, box_inner, box_outer);
 }
 
+// [batches][rows][ld] memory: a box never runs from one batch into the next
+// (rows past the end of a batch read as zeros).
+bool tma_map_bf16_3d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t rows,
+                     uint64_t batches, uint64_t ld, uint32_t box_inner, uint32_t box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr || (reinterpret_cast<uintptr_t>(base) & 15) || (ld * 2) % 16) return false;
+  cuuint64_t dims[3] = {inner, rows, batches};
+  cuuint64_t strides[2] = {ld * 2, rows * ld * 2};
+  cuuint32_t box[3] = {box_inner, box_rows, 1};
+  cuuint32_t es[3] = {1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, es,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace ewb

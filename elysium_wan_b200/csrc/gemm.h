@@ -102,5 +102,7 @@ void set_gemm_pair_mode(int mode);
 // elements, ld = row pitch in elements); false if the driver refuses it.
 bool tma_map_bf16_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,
                      uint64_t ld, uint32_t box_inner, uint32_t box_outer);
+bool tma_map_bf16_3d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t rows,
+                     uint64_t batches, uint64_t ld, uint32_t box_inner, uint32_t box_rows);
 
 }  // namespace ewb

@@ -313,9 +313,11 @@ struct WindowAttnBwdArgs {
   WindowAttnArgs f;  // o and lse as the forward left them
   const __nv_bfloat16* dout;  // [B * S][ldo]
   int64_t ldo;
-  float* Dbuf;          // [B][H][S] scratch
+  float* ws;            // window_attention_bwd_ws(f) floats of scratch
   __nv_bfloat16* dqkv;  // [B * S][(H + 2 Hkv) hd]
 };
+int64_t window_attention_bwd_ws(const WindowAttnArgs& f);
+int window_attention_bwd_launches(const WindowAttnArgs& f);
 int window_attention_bwd(const WindowAttnBwdArgs& a, cudaStream_t stream);
 
 }  // namespace ewb

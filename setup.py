@@ -26,7 +26,8 @@ for var, path in (("CC", "/usr/bin/gcc"), ("CXX", "/usr/bin/g++")):
 CSRC = os.path.join("elysium_wan_b200", "csrc")
 CU = ["gemm.cu", "norm.cu", "attention.cu", "ce.cu", "embed.cu", "optim.cu", "misc.cu",
       "collectives.cu", "llama.cu", "attention_tc.cu",
-      "dropout.cu", "logprobs.cu", "window_step.cu"]
+      "dropout.cu", "logprobs.cu", "window_step.cu", "window_attention.cu",
+      "window_attention_bwd.cu"]
 
 NVCC = [
     "-gencode", "arch=compute_100a,code=sm_100a",

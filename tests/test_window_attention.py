@@ -1,0 +1,265 @@
+"""Attention in a sliding window with sinks, forward and backward.
+
+Would fail if: a tile's mask (window edge, sinks, diagonal, length) were off by
+one, a row without a visible key or past a length gave anything but 0, NaN in
+padding reached a sum, a head width's ragged chunk were misread, a kv head's
+gradient missed a query head, the split of the sinks' tiles lost a part, rows of
+one sequence saw another's, or strides were ignored.
+"""
+
+import math
+
+import pytest
+import torch
+
+from elysium_wan_b200 import ops
+
+INF = math.inf
+U = 2.0**-8  # unit roundoff of bf16
+
+
+def plain64(qkv, dout, B, S, H, hd, Hkv, window, sinks, lengths=None):
+    """Everything in 64 bits, with bounds on what bf16 weights and outputs may
+    change: dict of name -> (value, bound), in [B, S, heads, hd] layout."""
+    x = qkv.double().view(B, S, H + 2 * Hkv, hd).transpose(1, 2)
+    do = dout.double().view(B, S, H, hd).transpose(1, 2)
+    i, j = torch.arange(S, device=x.device)[:, None], torch.arange(S, device=x.device)[None]
+    seen = ((j <= i) & ((i - j < window) | (j < sinks)))[None, None]
+    if lengths is not None:
+        n = lengths.clamp(0, S).view(-1, 1, 1, 1).to(x.device)
+        inside = torch.arange(S, device=x.device)[:, None] < n
+        x, do = torch.where(inside, x, 0.0), torch.where(inside, do, 0.0)
+        seen = seen & (i < n) & (j < n)
+    rep = H // Hkv
+    q, k, v = x[:, :H], x[:, H:H + Hkv].repeat_interleave(rep, 1), x[:, H + Hkv:].repeat_interleave(rep, 1)
+    c = 1 / math.sqrt(hd)
+    s = (q @ k.mT * c).masked_fill(~seen, -INF)
+    lse = torch.logsumexp(s, -1)
+    p = torch.exp(s - torch.where(lse == -INF, 0.0, lse)[..., None])
+    o = p @ v
+    # weights are rounded to bf16 once, the output once; fp32 sums: 1e-5 of the terms
+    o_err = U * o.abs() + (U + 1e-5) * (p @ v.abs())
+    dp = do @ v.mT
+    D = (do * o).sum(-1, keepdim=True)
+    # D is taken from the rounded o
+    D_err = (do.abs() * o_err).sum(-1, keepdim=True) + 1e-5 * (do * o).abs().sum(-1, keepdim=True)
+    ds = p * (dp - D)
+    ds_err = U * ds.abs() + p * D_err + 1e-4 * p * (do.abs() @ v.abs().mT)
+    group = lambda t: t.view(B, Hkv, rep, S, hd).sum(2)  # noqa: E731
+    dq, dk, dv = ds @ k * c, group(ds.mT @ q) * c, group(p.mT @ do)
+    dq_err = U * dq.abs() + ds_err @ k.abs() * c
+    dk_err = U * dk.abs() + group(ds_err.mT @ q.abs()) * c
+    dv_err = U * dv.abs() + (U + 1e-4) * group(p.mT @ do.abs())
+    return {"o": (o, o_err), "lse": (lse / math.log(2), None), "dq": (dq, dq_err), "dk": (dk, dk_err),
+            "dv": (dv, dv_err)}
+
+
+def split(dqkv, B, S, H, hd, Hkv):
+    x = dqkv.view(B, S, H + 2 * Hkv, hd).transpose(1, 2)
+    return {"dq": x[:, :H], "dk": x[:, H:H + Hkv], "dv": x[:, H + Hkv:]}
+
+
+def inputs(B, S, H, hd, Hkv, dev, lengths=None, dtype=torch.bfloat16, junk=math.nan, seed=0):
+    g = torch.Generator(device=dev)
+    g.manual_seed(seed + S)
+    qkv = torch.randn(B * S, (H + 2 * Hkv) * hd, generator=g, device=dev).to(dtype)
+    dout = torch.randn(B * S, H * hd, generator=g, device=dev).to(dtype)
+    if lengths is not None:  # what lies past a length must not matter
+        past = (torch.arange(S)[None] >= lengths[:, None]).view(-1).to(dev)
+        qkv[past] = junk
+        dout[past] = junk
+    return qkv, dout
+
+
+def check(qkv, dout, B, S, H, hd, Hkv, window, sinks, lengths=None, slack=1.05):
+    kw = dict(window=window, sinks=sinks, lengths=None if lengths is None else lengths.to(qkv.device))
+    o, lse = ops.window_attention_fwd(qkv, B, S, H, hd, Hkv, **kw)
+    d = ops.window_attention_bwd(qkv, o, dout, lse, B, S, H, hd, Hkv, **kw)
+    if qkv.is_cuda:
+        assert ops.ext().status_record()[0] == 0
+    want = plain64(qkv, dout, B, S, H, hd, Hkv, window, sinks, lengths)
+    got = dict(o=o.view(B, S, H, hd).transpose(1, 2), lse=lse, **split(d, B, S, H, hd, Hkv))
+    for name, (w, err) in want.items():
+        a = got[name].double()
+        if err is None:
+            err = 3e-5 * (1.0 + w.abs())
+        bad = ~((a == w) | ((a - w).abs() <= slack * err + 1e-6))
+        assert not bool(bad.any()), (name, bad.nonzero()[:4].tolist(), a[bad][:4], w[bad][:4])
+    if lengths is not None:
+        past = (torch.arange(S)[None] >= lengths[:, None]).to(qkv.device)
+        assert bool((o.view(B, S, -1)[past] == 0).all()) and bool((d.view(B, S, -1)[past] == 0).all())
+        assert bool((lse.transpose(1, 2)[past] == -INF).all())
+    return o, lse, d
+
+
+def test_host_path():
+    lengths = torch.tensor([9, 0, 23], dtype=torch.int32)
+    for window, sinks in ((1, 0), (4, 2), (30, 0), (5, 23)):
+        qkv, dout = inputs(3, 23, 4, 8, 2, "cpu", dtype=torch.float32)
+        check(qkv, dout, 3, 23, 4, 8, 2, window, sinks)
+        qkv, dout = inputs(3, 23, 4, 8, 2, "cpu", lengths, torch.float32)
+        check(qkv, dout, 3, 23, 4, 8, 2, window, sinks, lengths)
+
+
+def test_host_full_window_is_causal_attention():
+    qkv, dout = inputs(2, 16, 4, 8, 2, "cpu", dtype=torch.float32)
+    o, lse = ops.attention_fwd(qkv, 2, 16, 4, 8, 2)
+    w = ops.window_attention_fwd(qkv, 2, 16, 4, 8, 2, window=16)
+    assert torch.allclose(w[0], o, atol=1e-6) and torch.allclose(w[1], lse, atol=1e-5)
+    d = ops.attention_bwd(qkv, o, dout, lse, 2, 16, 4, 8, 2)
+    assert torch.allclose(ops.window_attention_bwd(qkv, *w[:1], dout, w[1], 2, 16, 4, 8, 2, window=16), d,
+                          atol=1e-5)
+
+
+def test_host_gradient_against_differences():
+    B, S, H, hd, Hkv = 2, 7, 4, 8, 2
+    qkv, dout = inputs(B, S, H, hd, Hkv, "cpu", dtype=torch.float32)
+    lengths = torch.tensor([7, 4], dtype=torch.int32)
+    kw = dict(window=3, sinks=1, lengths=lengths)
+    o, lse = ops.window_attention_fwd(qkv, B, S, H, hd, Hkv, **kw)
+    d = ops.window_attention_bwd(qkv, o, dout, lse, B, S, H, hd, Hkv, **kw)
+    for row, col in ((0, 0), (1, 33), (6, 50), (7, 5), (10, 63), (9, 40)):
+        f = []
+        for h in (1e-4, -1e-4):
+            x = qkv.double().clone()
+            x[row, col] += h
+            f.append((plain64(x, dout, B, S, H, hd, Hkv, 3, 1, lengths)["o"][0].transpose(1, 2).reshape(B * S, -1)
+                      * dout.double()).sum())
+        # the difference's own error: h^2 times a third derivative of size 1 to 10
+        assert abs((f[0] - f[1]) / 2e-4 - d[row, col]) < 2e-5 * (1 + abs(d[row, col]))
+
+
+def test_refusals_host():
+    x = torch.zeros(6, 64)
+    for bad in (dict(window=0), dict(window=2, sinks=-1)):
+        with pytest.raises(ValueError):
+            ops.window_attention_fwd(x, 2, 3, 4, 8, 2, **bad)
+    for shape in ((2, 2, 4, 8, 2), (2, 3, 3, 8, 2), (2, 3, 4, 8, 4)):
+        with pytest.raises(ValueError):
+            ops.window_attention_fwd(x, *shape, window=2)
+
+
+# ----------------------------------------------------------------------------- GPU
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 80, 96, 128])
+@pytest.mark.parametrize("S", [1, 5, 64, 127, 128, 129, 256, 257, 400])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (60, 3), (128, 0), (129, 129), (1000, 0)])
+def test_gpu_lengths_and_windows(cuda, hd, S, window, sinks):
+    qkv, dout = inputs(2, S, 3, hd, 3, cuda)
+    check(qkv, dout, 2, S, 3, hd, 3, window, sinks)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S,window,sinks", [(1500, 1, 1), (1500, 100, 4), (1500, 256, 300), (1500, 700, 0),
+                                            (1411, 130, 130), (2048, 64, 1)])
+@pytest.mark.parametrize("H,Hkv,hd", [(4, 1, 128), (2, 2, 64), (6, 2, 80)])
+def test_gpu_long(cuda, S, window, sinks, H, Hkv, hd):
+    qkv, dout = inputs(1, S, H, hd, Hkv, cuda)
+    check(qkv, dout, 1, S, H, hd, Hkv, window, sinks)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 80, 128])
+@pytest.mark.parametrize("window,sinks", [(50, 2), (200, 0), (10000, 0), (3, 140)])
+def test_gpu_padding_is_never_used(cuda, hd, window, sinks):
+    """NaN past every length: empty, one token, inside, at and around a tile's end."""
+    S = 300
+    lengths = torch.tensor([300, 0, 1, 63, 64, 65, 128, 129, 255, 257, 299], dtype=torch.int32)
+    B = len(lengths)
+    qkv, dout = inputs(B, S, 2, hd, 1, cuda, lengths)
+    check(qkv, dout, B, S, 2, hd, 1, window, sinks, lengths)
+    wild = lengths.clone()  # values outside [0, S] count as the nearer bound
+    wild[0], wild[1] = 5000, -3
+    a = ops.window_attention_fwd(qkv, B, S, 2, hd, 1, window=window, sinks=sinks, lengths=wild.to(cuda))
+    b = ops.window_attention_fwd(qkv, B, S, 2, hd, 1, window=window, sinks=sinks, lengths=lengths.to(cuda))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.gpu
+def test_gpu_strided_rows(cuda):
+    """qkv and dout as slices of wider rows give the dense result, bit for bit."""
+    B, S, H, hd, Hkv = 2, 200, 4, 64, 2
+    big = torch.randn(B * S, 8 * 64 + 24, device=cuda).to(torch.bfloat16)
+    dbig = torch.randn(B * S, 4 * 64 + 8, device=cuda).to(torch.bfloat16)
+    qkv, dout = big[:, 16:16 + 8 * 64], dbig[:, 8:]
+    a = check(qkv, dout, B, S, H, hd, Hkv, 70, 5)
+    b = check(qkv.contiguous(), dout.contiguous(), B, S, H, hd, Hkv, 70, 5)
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+def test_gpu_deterministic_and_independent_sequences(cuda):
+    B, S, H, hd, Hkv = 3, 700, 8, 128, 2
+    qkv, dout = inputs(B, S, H, hd, Hkv, cuda)
+    one = check(qkv, dout, B, S, H, hd, Hkv, 150, 4)
+    two = check(qkv, dout, B, S, H, hd, Hkv, 150, 4)
+    for x, y in zip(one, two):
+        assert torch.equal(x, y)
+    rows = slice(S, 2 * S)
+    alone = check(qkv[rows], dout[rows], 1, S, H, hd, Hkv, 150, 4)
+    assert torch.equal(alone[0], one[0][rows]) and torch.equal(alone[2], one[2][rows])
+
+
+@pytest.mark.gpu
+def test_gpu_large_scores(cuda):
+    """Scores of several hundred: the running maximum has to move many times."""
+    B, S, H, hd, Hkv = 1, 600, 2, 128, 2
+    qkv, dout = inputs(B, S, H, hd, Hkv, cuda)
+    qkv = (qkv.float() * torch.linspace(0.3, 6.0, S, device=cuda)[:, None]).to(torch.bfloat16)
+    kw = dict(window=256, sinks=3)
+    o, lse = ops.window_attention_fwd(qkv, B, S, H, hd, Hkv, **kw)
+    want = plain64(qkv, dout, B, S, H, hd, Hkv, 256, 3)
+    # weights carry the fp32 scores' error, |x| 2^-22 for scores up to 500
+    w, err = want["o"]
+    v = qkv.double().view(B, S, -1, hd).transpose(1, 2)[:, H + Hkv:].abs().amax()
+    assert bool(((o.view(B, S, H, hd).transpose(1, 2).double() - w).abs() <= 1.05 * err + 5e-4 * v).all())
+    assert bool(((lse.double() - want["lse"][0]).abs() <= 3e-5 * (1 + want["lse"][0].abs())).all())
+
+
+@pytest.mark.gpu
+def test_gpu_other_stream_and_wide_batch(cuda):
+    B, S, H, hd, Hkv = 70, 33, 2, 64, 1
+    qkv, dout = inputs(B, S, H, hd, Hkv, cuda)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        a = ops.window_attention_fwd(qkv, B, S, H, hd, Hkv, window=9, sinks=1)
+    s.synchronize()
+    b = check(qkv, dout, B, S, H, hd, Hkv, 9, 1)
+    assert torch.equal(a[0], b[0])
+
+
+@pytest.mark.gpu
+def test_gpu_refusals(cuda):
+    B, S, H, hd, Hkv = 2, 5, 4, 64, 2
+    qkv, dout = inputs(B, S, H, hd, Hkv, cuda)
+    fwd, shape = ops.window_attention_fwd, (B, S, H, hd, Hkv)
+    for bad in (dict(window=0), dict(window=2, sinks=-1)):
+        with pytest.raises(RuntimeError, match="window must"):
+            fwd(qkv, *shape, **bad)
+    with pytest.raises(RuntimeError, match="head width"):
+        fwd(qkv, B, S, 8, 32, 4, window=2)
+    with pytest.raises(RuntimeError, match="q . k . v"):
+        fwd(qkv, B, S, H, hd, 4, window=2)
+    with pytest.raises(RuntimeError, match="multiple of Hkv"):
+        fwd(qkv, B, S, 5, 64, 3, window=2)
+    with pytest.raises(RuntimeError, match="B . S rows"):
+        fwd(qkv, B, S + 1, H, hd, Hkv, window=2)
+    with pytest.raises(RuntimeError, match="bf16"):
+        fwd(qkv.float(), *shape, window=2)
+    with pytest.raises(RuntimeError, match="aligned"):
+        wide = torch.zeros(B * S, qkv.shape[1] + 1, device=cuda, dtype=torch.bfloat16)
+        fwd(wide[:, 1:], *shape, window=2)
+    with pytest.raises(RuntimeError, match="int32"):
+        fwd(qkv, *shape, window=2, lengths=torch.zeros(B, device=cuda, dtype=torch.int64))
+    with pytest.raises(RuntimeError, match="must be on"):
+        fwd(qkv, *shape, window=2, lengths=torch.zeros(B, dtype=torch.int32))
+    o, lse = fwd(qkv, *shape, window=2)
+    for args in ((o[:-1], dout, lse), (o, dout[:, :-8], lse), (o, dout, lse[:1]), (o.float(), dout, lse)):
+        with pytest.raises(RuntimeError):
+            ops.window_attention_bwd(qkv, *args, *shape, window=2)
+    e = qkv[:0]
+    o, lse = fwd(e, 0, S, H, hd, Hkv, window=2)
+    assert o.shape == (0, H * hd) and lse.shape == (0, H, S)
+    assert ops.window_attention_bwd(e, o, dout[:0], lse, 0, S, H, hd, Hkv, window=2).shape == e.shape

@@ -14,9 +14,161 @@ __device__ __forceinline__ float ex2_wa(float x) {
   return y;
 }
 
+// Pairs of fp32 values in one register pair: one instruction works on both.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair2(uint32_t lo, uint32_t hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+__device__ __forceinline__ f32x2 pair2(float lo, float hi) {
+  return pair2(__float_as_uint(lo), __float_as_uint(hi));
+}
+__device__ __forceinline__ void unpair2(f32x2 v, float& lo, float& hi) {
+  uint32_t a, b;
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
+  lo = __uint_as_float(a);
+  hi = __uint_as_float(b);
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 2^x of a pair on the FMA pipe, for x >= -126 (lower counts as -126): x = n + f
+// with n the nearest whole number, 2^f by a polynomial of degree 4 on [-1/2,
+// 1/2] (a weighted least-squares fit made minimax by reweighting, with 1 at f = 0;
+// relative error 2.8e-6), n added to the exponent. It takes a share of the
+// exponentials off the special-function unit (16 a cycle on an SM).
+__device__ __forceinline__ void ex2_poly2(f32x2 x, float& p0, float& p1) {
+  float a, b;
+  unpair2(x, a, b);
+  x = pair2(fmaxf(a, -126.f), fmaxf(b, -126.f));
+  const f32x2 magic = pair2(12582912.f, 12582912.f), back = pair2(-12582912.f, -12582912.f);
+  const f32x2 t = add2(x, magic);  // n in the low bits
+  const f32x2 f = fma2(add2(t, back), pair2(-1.f, -1.f), x);
+  f32x2 p = fma2(f, pair2(0.00958285295f, 0.00958285295f), pair2(0.0559064262f, 0.0559064262f));
+  p = fma2(p, f, pair2(0.240240991f, 0.240240991f));
+  p = fma2(p, f, pair2(0.693124175f, 0.693124175f));
+  p = fma2(p, f, pair2(1.f, 1.f));
+  float t0, t1;
+  unpair2(t, t0, t1);
+  unpair2(p, p0, p1);
+  p0 = __int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23));
+  p1 = __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23));
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// A shared-memory descriptor (sdesc_sw128) moved by `bytes`. One thread issues
+// all MMAs, so what it does between two of them counts: the descriptor of a tile
+// is made once, and its steps only add to the address field (which cannot carry
+// into the next one: shared memory ends below 2^18).
+__device__ __forceinline__ uint64_t desc_at(uint64_t d, uint32_t bytes) {
+  uint64_t r;
+  asm("{\n\t.reg .b32 lo, hi;\n\tmov.b64 {lo, hi}, %1;\n\tadd.u32 lo, lo, %2;\n\tmov.b64 %0, {lo, hi};\n\t}"
+      : "=l"(r)
+      : "l"(d), "r"(bytes >> 4));
+  return r;
+}
+
+// MMA issue by one lane of a converged warp: the warp's control flow and operands
+// stay uniform, so descriptors live in uniform registers, where the MMA wants
+// them. With the loop itself inside a one-lane branch each MMA took 80 to 95
+// cycles instead of the 64 that its 128 x 128 x 16 products need.
+__device__ __forceinline__ uint32_t elect_lane() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p;
+}
+__device__ __forceinline__ void umma_ss(uint32_t lead, uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(lead)
+      : "memory");
+}
+// A (128 rows x 16, two bf16 a column) in TMEM.
+__device__ __forceinline__ void umma_ts(uint32_t lead, uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void umma_commit_by(uint32_t lead, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(lead)
+      : "memory");
+}
+// A wait of a whole warp, with one answer for all of it.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* status, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, code));
+}
+
+// Cluster launch control: a running CTA takes the place of one that has not
+// been launched yet, and with it its block index. The answer (16 bytes of
+// shared memory) completes on `bar`. A CTA that got "none left" must not ask again.
+__device__ __forceinline__ void next_block_ask(void* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_u32(answer)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+// The block index (x) of the answer, or -1 for none left.
+__device__ __forceinline__ int next_block_read(const void* answer) {
+  int x;
+  asm volatile(
+      "{\n\t.reg .b128 a;\n\t.reg .b64 lo, hi;\n\t.reg .pred p;\n\t"
+      "ld.shared.v2.b64 {lo, hi}, [%1];\n\tmov.b128 a, {lo, hi};\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\t"
+      "mov.b32 %0, -1;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, a;\n\t}"
+      : "=&r"(x)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return x;
+}
+
+template <int N>
+__device__ __forceinline__ void reg_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void reg_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 // Bits c < n of a 32-bit word.
 __device__ __forceinline__ uint32_t bits_below(int n) {
   return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+}
+
+// -inf in the places of v whose bit is not set.
+__device__ __forceinline__ void mask32(uint32_t* v, uint32_t bits) {
+  if (__all_sync(0xffffffffu, bits == 0xffffffffu)) return;
+#pragma unroll
+  for (int e = 0; e < 32; ++e)
+    if (!((bits >> e) & 1u)) v[e] = 0xff800000u;
 }
 
 // The key tiles (128 keys) that the rows [q0, q1] can see: [0, ns) and [w0, e].

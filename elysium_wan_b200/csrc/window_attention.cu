@@ -4,24 +4,29 @@
 //
 //   x = q k / sqrt(hd);  p = e^(x - m);  o = sum p v / sum p;  lse2 = log2 sum e^x
 //
-// One CTA owns 256 query rows of one (batch, head) as two subtiles of 128 and
-// walks the key tiles of 128 that either can see: the sinks' tiles, then the
-// window's. Each K and V tile is loaded once for both subtiles, which halves the
-// traffic from the L2 (at 128 rows a CTA it would bound the kernel: 64 KB for
-// 1024 cycles of tensor work on each SM). Ten warps:
-//   warp 0     TMA producer: Q once, then K and V tiles into their rings;
-//   warp 1     MMA issuer (one thread): for each tile k and subtile t,
+// A block is an item: 256 query rows of one (batch, head). A CTA stays on its SM and
+// takes over blocks not yet launched (cluster launch control), so that loads of
+// the next item run under the end of this one; it works on an item as
+// two subtiles of 128, and walks the key tiles of 128 that either can see: the
+// sinks' tiles, then the window's. Each K and V tile is loaded once for both
+// subtiles, which halves the traffic from the L2 (at 128 rows an item it would
+// bound the kernel: 64 KB for 1024 cycles of tensor work on each SM). Twelve warps:
+//   warp 0     TMA producer: Q, then K and V tiles into their rings, running
+//              ahead into the next item;
+//   warp 1     MMA issuer: for each tile k and subtile t,
 //              O_t += P_t V_{k-1}, then S_t = Q_t K_k^T over the same TMEM columns
 //              (MMAs of one thread run in order, so S_t may overwrite P_t);
-//   warps 2-5, 6-9  softmax of subtile 0 and 1, one query row a thread: while
-//              one subtile is in the tensor cores the other one is here.
-// P never leaves TMEM: the softmax thread reads its row of S, and writes the
+//   warp 2     asks for the next block;
+//   warps 4-7, 8-11  softmax of subtile 0 and 1, one query row a thread. While one
+//              subtile is in the tensor cores the other one is here.
+// P never leaves TMEM: the softmax thread reads its row of S and writes the
 // row's bf16 weights over the first half of the same columns, from where the
-// second product reads them as its A operand. The running maximum moves only
-// when it grows by more than 2^8 (weights and sums share it, so o is unchanged),
-// and then the same thread rescales its row of O: S_t is complete only after
-// every earlier product of this CTA, so O_t rests meanwhile.
-// TMEM: S_0 | S_1 | O_0 | O_1 = 512 columns. Shared memory: Q 2 tiles, K 2, V 3.
+// second product reads them as its A operand.
+// The running maximum moves only when it grows by more than 2^8 (weights and sums
+// share it, so o is unchanged), and then the same threads rescale their row of O:
+// S_t is complete only after every earlier product of this CTA, so O_t rests
+// meanwhile.
+// TMEM: S_0 | S_1 | O_0 | O_1 = 512 columns. Shared memory: Q, K, V 2 tiles each.
 //
 // Rows past a sequence's end: boxes of the 3D tensor map read zeros past S; the
 // V tile that holds the end of a shorter sequence is cleared from there on by
@@ -36,76 +41,141 @@
 namespace ewb {
 namespace {
 
-constexpr int kWaKStages = 2, kWaVStages = 3;
-constexpr int kWaThreads = 320;
+constexpr int kWaStages = 2;
+constexpr int kWaThreads = 384;
+// registers a thread: 88 + 2 x 208 = 3 x 168, what the launch takes
+constexpr int kWaRegsIssue = 88, kWaRegsSoftmax = 208;
 constexpr float kWaRescale = 8.0f;
 
 template <int HD>
 struct WaLayout {
   static constexpr int kChunks = HeadChunks<HD>::kCount;
   static constexpr uint32_t kTile = kChunks * kWaChunk;
-  static constexpr uint32_t kQ = 0, kK = 2 * kTile, kV = kK + kWaKStages * kTile;
-  static constexpr uint32_t kBar = kV + kWaVStages * kTile;
-  static constexpr int kSmem = static_cast<int>(kBar) + 256 + 1024;
+  static constexpr uint32_t kQ = 0, kK = 2 * kTile, kV = kK + kWaStages * kTile;
+  static constexpr uint32_t kStage = kV + kWaStages * kTile;  // 32 rows x 128 bytes a softmax warp
+  static constexpr uint32_t kBar = kStage + 8 * 4096;
+  static constexpr int kSmem = static_cast<int>(kBar) + 512 + 1024;
 };
+
+// What every role has to know of one item.
+struct WaItem {
+  int h, b, hk, q0, n;
+  int live;   // subtiles with a row below the length
+  int tiles;  // key tiles of the item
+  TileList all, sub0, sub1;
+  __device__ __forceinline__ WaItem(int w, int B, int H, int rep, int S, int blocks, int window, int sinks,
+                                    const int* lengths)
+      : all(0, 0, 1, 0), sub0(0, 0, 1, 0), sub1(0, 0, 1, 0) {
+    h = w % H;
+    w /= H;
+    b = w % B;
+    q0 = (blocks - 1 - w / B) * 256;  // the latest rows first: most tiles
+    hk = h / rep;
+    n = lengths != nullptr ? min(max(lengths[b], 0), S) : S;
+    n = __shfl_sync(0xffffffffu, n, 0);  // the same in every lane, and known to be
+    live = n <= q0 ? 0 : n <= q0 + 128 ? 1 : 2;
+    const int last = max(n, 1) - 1;
+    all = TileList(q0, min(q0 + 255, last), window, sinks);
+    sub0 = TileList(q0, min(q0 + 127, last), window, sinks);
+    sub1 = TileList(q0 + 128, min(q0 + 255, last), window, sinks);
+    tiles = live > 0 ? all.count() : 0;
+  }
+  // does subtile t see tile j?
+  __device__ __forceinline__ bool sees(int t, int j) const {
+    const TileList& s = t ? sub1 : sub0;
+    return t < live && (j < s.ns || j >= s.w0) && j <= s.e;
+  }
+};
+
+// The items of a CTA: its own block index, then those of blocks that it takes
+// over (next_block_ask), one asked for ahead. Every warp that works on items
+// walks them with one of these.
+struct WaQueue {
+  const void* answer;
+  uint64_t *full, *empty;
+  int seen = 0;
+  // The next item after `w`; -1: none left (or a wait ran out).
+  __device__ __forceinline__ int next(int* status, int lane) {
+    if (!warp_wait(full, seen & 1, status, kStatusTimeoutSmemFull)) return -1;
+    const int w = __shfl_sync(0xffffffffu, next_block_read(answer), 0);
+    ++seen;
+    fence_proxy_async_smem();  // read before the next answer is written over it
+    __syncwarp();
+    if (lane == 0) mbar_arrive(empty);
+    return w;
+  }
+};
+
+// 32 weights 2^(x scale - base) of a row as bf16 pairs, and their sums in fp32.
+// One pair in four goes to the FMA pipe: a warp's 128 columns take 1250 cycles
+// alone on its scheduler so, 1420 on the special-function unit alone, 1280 with
+// one in two.
+__device__ __forceinline__ void row_weights(const uint32_t* v, f32x2 scale2, f32x2 minus2, uint32_t* pk,
+                                            f32x2* sum) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const f32x2 x = fma2(pair2(v[2 * e], v[2 * e + 1]), scale2, minus2);
+    float p0, p1;
+    if (e % 4 == 3) {
+      ex2_poly2(x, p0, p1);
+    } else {
+      unpair2(x, p0, p1);
+      p0 = ex2_wa(p0);
+      p1 = ex2_wa(p1);
+    }
+    sum[e & 3] = add2(sum[e & 3], pair2(p0, p1));
+    pk[e] = pack_bf16x2(p0, p1);
+  }
+}
 
 template <int HD>
 __global__ void __launch_bounds__(kWaThreads, 1)
     window_fwd_kernel(const __grid_constant__ CUtensorMap map, __nv_bfloat16* __restrict__ o,
-                      float* __restrict__ lse2, const int* __restrict__ lengths, int S, int H,
+                      float* __restrict__ lse2, const int* __restrict__ lengths, int B, int S, int H,
                       int Hkv, int window, int sinks, float scale_log2, int* status) {
   using L = WaLayout<HD>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
-  uint64_t* qfull = bars;                       // [2]
-  uint64_t* kfull = qfull + 2;                  // [kWaKStages]
-  uint64_t* kempty = kfull + kWaKStages;
-  uint64_t* vfull = kempty + kWaKStages;        // [kWaVStages]
-  uint64_t* vempty = vfull + kWaVStages;
-  uint64_t* sfull = vempty + kWaVStages;        // [2]
-  uint64_t* pfull = sfull + 2;                  // [2]
-  uint64_t* ofull = pfull + 2;                  // [2]
-  uint64_t* landed = ofull + 2;                 // the V tile that the producer clears
-  uint64_t* drain = landed + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint64_t* qfull = bars;         // [2]
+  uint64_t* qempty = bars + 2;    // [2]
+  uint64_t* kfull = bars + 4;     // [2]
+  uint64_t* kempty = bars + 6;    // [2]
+  uint64_t* vfull = bars + 8;     // [2]
+  uint64_t* vempty = bars + 10;   // [2]
+  uint64_t* sfull = bars + 12;    // [2]
+  uint64_t* pfull = bars + 14;    // [2][2]: keys 0-95 and 96-127 of P_t
+  uint64_t* ofull = bars + 18;    // [2]
+  uint64_t* ofree = bars + 20;    // [2] O_t read by the softmax warps
+  uint64_t* landed = bars + 22;   // a V tile that the producer clears
+  uint64_t* drain = bars + 23;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
+  uint64_t* wfull = bars + 26;   // the next item's index
+  uint64_t* wempty = bars + 27;  // read by the producer, the MMA warp and the softmax warps
+  uint64_t* answer = bars + 28;  // [2]
 
-  const int h = blockIdx.x, b = blockIdx.z;
-  const int q0 = (gridDim.y - 1 - blockIdx.y) * 256;  // the latest rows first: most tiles
-  const int hk = h / (H / Hkv);
-  const int n = lengths != nullptr ? min(max(lengths[b], 0), S) : S;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // subtile t: rows q0 + 128 t ..; none of them below the length: no work
-  const int live = n <= q0 ? 0 : n <= q0 + 128 ? 1 : 2;
-  const TileList all(q0, min(q0 + 255, max(n, 1) - 1), window, sinks);
-  const TileList sub0(q0, min(q0 + 127, max(n, 1) - 1), window, sinks);
-  const TileList sub1(q0 + 128, min(q0 + 255, max(n, 1) - 1), window, sinks);
-  const int tiles = live > 0 ? all.count() : 0;
-  // does subtile t see tile j?
-  auto sees = [&](int t, int j) -> bool {
-    if (t >= live) return false;
-    const TileList& s = t ? sub1 : sub0;
-    return (j < s.ns || j >= s.w0) && j <= s.e;
-  };
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int rep = H / Hkv, blocks = (S + 255) / 256;
 
   if (warp == 0 && lane == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&qfull[i], 1);
-      mbar_init(&sfull[i], 1);
-      mbar_init(&pfull[i], 4);
-      mbar_init(&ofull[i], 1);
-    }
-    for (int i = 0; i < kWaKStages; ++i) {
+      mbar_init(&qempty[i], 1);
       mbar_init(&kfull[i], 1);
       mbar_init(&kempty[i], 1);
-    }
-    for (int i = 0; i < kWaVStages; ++i) {
       mbar_init(&vfull[i], 1);
       mbar_init(&vempty[i], 1);
+      mbar_init(&sfull[i], 1);
+      mbar_init(&pfull[2 * i], 4);
+      mbar_init(&pfull[2 * i + 1], 4);
+      mbar_init(&ofull[i], 1);
+      mbar_init(&ofree[i], 4);
     }
     mbar_init(landed, 1);
     mbar_init(drain, 1);
+    mbar_init(wfull, 1);
+    mbar_init(wempty, 10);
     fence_mbar_init();
     tma_prefetch_desc(&map);
   }
@@ -116,231 +186,327 @@ __global__ void __launch_bounds__(kWaThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
-  if (warp == 0) {
-    // The V tile that holds row n of a sequence shorter than S is cleared
-    // from that row on before it is handed over.
-    const int clear = (n < S && (n & 127)) ? n >> 7 : -1;
-    const int kcol = (H + hk) * HD, vcol = (H + Hkv + hk) * HD;
-    bool ok = true;
-    int kdone = 0, vdone = 0;  // tiles whose loads were issued
-    if (lane == 0) {
-      for (int t = 0; t < live; ++t) {
-        mbar_arrive_expect_tx(&qfull[t], L::kTile);
-        for (int c = 0; c < L::kChunks; ++c)
-          tma_load_3d(smem + L::kQ + t * L::kTile + c * kWaChunk, &map, &qfull[t], h * HD + c * 64,
-                      q0 + t * 128, b, status);
-      }
-    }
-    for (int k = 0; k < tiles && ok; ++k) {
-      const int j = all.tile(k);
-      const int ks = k % kWaKStages, vs = k % kWaVStages;
-      uint8_t* sv = smem + L::kV + vs * L::kTile;
-      uint64_t* vbar = j == clear ? landed : &vfull[vs];
-      if (lane == 0) {
-        ok = mbar_wait(&kempty[ks], ((k / kWaKStages) & 1) ^ 1, status, kStatusTimeoutSmemEmpty);
-        if (ok) {
-          mbar_arrive_expect_tx(&kfull[ks], L::kTile);
-          for (int c = 0; c < L::kChunks; ++c)
-            tma_load_3d(smem + L::kK + ks * L::kTile + c * kWaChunk, &map, &kfull[ks], kcol + c * 64,
-                        j * 128, b, status);
-          kdone = k + 1;
-          ok = mbar_wait(&vempty[vs], ((k / kWaVStages) & 1) ^ 1, status, kStatusTimeoutSmemEmpty);
+  WaQueue queue{answer, wfull, wempty};
+  if (warp < 4) {
+    reg_dec<kWaRegsIssue>();
+    if (warp == 2) {
+      // asks for the next item once every role has taken the one before
+      for (int i = 0;; ++i) {
+        if (!warp_wait(wempty, (i & 1) ^ 1, status, kStatusTimeoutSmemEmpty)) {
+          // nothing is asked for: the roles' own waits end
+          break;
         }
-        if (ok) {
-          mbar_arrive_expect_tx(vbar, L::kTile);
-          for (int c = 0; c < L::kChunks; ++c)
-            tma_load_3d(sv + c * kWaChunk, &map, vbar, vcol + c * 64, j * 128, b, status);
-          vdone = k + 1;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(wfull, 16);
+          next_block_ask(answer, wfull);
         }
-      }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
-      if (ok && j == clear) {
-        if (!mbar_wait(landed, 0, status, kStatusTimeoutSmemFull)) ok = false;
-        ok = __all_sync(0xffffffffu, ok);
-        const int r0 = n & 127;
-        for (int i = lane; i < (128 - r0) * 8 * L::kChunks; i += 32) {
-          const int c = i / ((128 - r0) * 8), w = i - c * (128 - r0) * 8;
-          *reinterpret_cast<uint4*>(sv + c * kWaChunk + r0 * 128 + w * 16) = make_uint4(0, 0, 0, 0);
-        }
-        fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&vfull[vs]);
+        if (!warp_wait(wfull, i & 1, status, kStatusTimeoutSmemFull)) {
+          mbar_wait(wfull, i & 1, nullptr, kStatusTimeoutDrain);  // the answer must land
+          break;
+        }
+        if (__shfl_sync(0xffffffffu, next_block_read(answer), 0) < 0) break;
       }
-    }
-    // Loads already issued must land before this CTA's memory goes away.
-    if (lane == 0) {
-      for (int t = 0; t < live; ++t) mbar_wait(&qfull[t], 0, nullptr, kStatusTimeoutDrain);
-      for (int k = kdone - 1; k >= 0 && k >= kdone - kWaKStages; --k)
-        mbar_wait(&kfull[k % kWaKStages], (k / kWaKStages) & 1, nullptr, kStatusTimeoutDrain);
-      for (int k = vdone - 1; k >= 0 && k >= vdone - kWaVStages; --k) {
-        if (all.tile(k) == clear) mbar_wait(landed, 0, nullptr, kStatusTimeoutDrain);
-        else mbar_wait(&vfull[k % kWaVStages], (k / kWaVStages) & 1, nullptr, kStatusTimeoutDrain);
+    } else if (warp == 0) {
+      bool ok = true;
+      int kv = 0, qn[2] = {0, 0}, cleared = 0;  // K / V tiles, Q subtiles, cleared tiles so far
+      int last_cleared = -1;                    // the last of them, as a number of kv
+      for (int w = blockIdx.x; w >= 0 && ok; w = queue.next(status, lane)) {
+        const WaItem a(w, B, H, rep, S, blocks, window, sinks, lengths);
+        // The V tile that holds row n of a sequence shorter than S is cleared
+        // from that row on before it is handed over.
+        const int clear = (a.n < S && (a.n & 127)) ? a.n >> 7 : -1;
+        const int kcol = (H + a.hk) * HD, vcol = (H + Hkv + a.hk) * HD;
+        for (int k = 0; k < a.tiles && ok; ++k) {
+          const int j = a.all.tile(k), s = kv % kWaStages;
+          const uint32_t ph = ((kv / kWaStages) & 1) ^ 1;
+          uint8_t* sv = smem + L::kV + s * L::kTile;
+          uint64_t* vbar = j == clear ? landed : &vfull[s];
+          auto load_q = [&](int t) {
+            ok = warp_wait(&qempty[t], (qn[t] & 1) ^ 1, status, kStatusTimeoutSmemEmpty);
+            if (!ok) return;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&qfull[t], L::kTile);
+              for (int c = 0; c < L::kChunks; ++c)
+                tma_load_3d(smem + L::kQ + t * L::kTile + c * kWaChunk, &map, &qfull[t], a.h * HD + c * 64,
+                            a.q0 + t * 128, a.b, status);
+            }
+            ++qn[t];
+          };
+          // subtile 0 of an item may start before subtile 1 of the last one ends
+          if (k == 0) load_q(0);
+          ok = ok && warp_wait(&kempty[s], ph, status, kStatusTimeoutSmemEmpty);
+          if (!ok) break;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&kfull[s], L::kTile);
+            for (int c = 0; c < L::kChunks; ++c)
+              tma_load_3d(smem + L::kK + s * L::kTile + c * kWaChunk, &map, &kfull[s], kcol + c * 64,
+                          j * 128, a.b, status);
+          }
+          if (k == 0 && a.live > 1) load_q(1);
+          ok = ok && warp_wait(&vempty[s], ph, status, kStatusTimeoutSmemEmpty);
+          if (!ok) {  // this K tile is on its way: let it land
+            mbar_wait(&kfull[s], (kv / kWaStages) & 1, nullptr, kStatusTimeoutDrain);
+            break;
+          }
+          if (lane == 0) {
+            mbar_arrive_expect_tx(vbar, L::kTile);
+            for (int c = 0; c < L::kChunks; ++c)
+              tma_load_3d(sv + c * kWaChunk, &map, vbar, vcol + c * 64, j * 128, a.b, status);
+          }
+          ++kv;
+          if (j == clear) {
+            ok = warp_wait(landed, cleared & 1, status, kStatusTimeoutSmemFull);
+            ++cleared;
+            last_cleared = kv - 1;
+            const int r0 = a.n & 127, per = (128 - r0) * 8;
+            for (int i = lane; i < per * L::kChunks; i += 32) {
+              const int c = i / per;
+              *reinterpret_cast<uint4*>(sv + c * kWaChunk + r0 * 128 + (i - c * per) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&vfull[s]);
+          }
+        }
       }
-    }
-  } else if (warp == 1) {
-    if (lane == 0) {
+      // Loads already issued must land before this CTA's memory goes away.
+      for (int t = 0; t < 2; ++t)
+        if (qn[t] > 0) mbar_wait(&qfull[t], (qn[t] - 1) & 1, nullptr, kStatusTimeoutDrain);
+      for (int k = kv - 1; k >= 0 && k >= kv - kWaStages; --k) {
+        mbar_wait(&kfull[k % kWaStages], (k / kWaStages) & 1, nullptr, kStatusTimeoutDrain);
+        if (k == last_cleared) mbar_wait(landed, (cleared - 1) & 1, nullptr, kStatusTimeoutDrain);
+        else mbar_wait(&vfull[k % kWaStages], (k / kWaStages) & 1, nullptr, kStatusTimeoutDrain);
+      }
+    } else if (warp == 1) {
+      const uint32_t lead = elect_lane();
       constexpr uint32_t IS = idesc_bf16_f32(128, 128, false, false);
       constexpr uint32_t IP = idesc_bf16_f32(128, HD, false, true);
-      const uint32_t q_addr = smem_u32(smem + L::kQ);
+      const uint64_t q_desc = sdesc_sw128(smem_u32(smem + L::kQ), 16, 1024);
+      const uint64_t k_desc0 = sdesc_sw128(smem_u32(smem + L::kK), 16, 1024);
+      const uint64_t v_desc0 = sdesc_sw128(smem_u32(smem + L::kV), kWaChunk, 1024);
       bool ok = true;
-      int done[2] = {0, 0};  // products P V issued
-      for (int t = 0; t < live; ++t) ok = ok && mbar_wait(&qfull[t], 0, status, kStatusTimeoutSmemFull);
-      for (int k = 0; k <= tiles && ok; ++k) {
-        if (tiles == 0) break;
-        const int j = all.tile(k), jp = k > 0 ? all.tile(k - 1) : 0;
-        const int ks = k % kWaKStages, vs = (k + kWaVStages - 1) % kWaVStages;
-        if (k < tiles)
-          ok = mbar_wait(&kfull[ks], (k / kWaKStages) & 1, status, kStatusTimeoutSmemFull);
-        if (ok && k > 0)
-          ok = mbar_wait(&vfull[vs], ((k - 1) / kWaVStages) & 1, status, kStatusTimeoutSmemFull);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t k_addr = smem_u32(smem + L::kK + ks * L::kTile);
-        const uint32_t v_addr = smem_u32(smem + L::kV + vs * L::kTile);
+      int kv = 0;             // tiles so far: parities of the K and V rings
+      int pn[2] = {0, 0};     // weights P_t used so far
+      int sn[2] = {0, 0};     // items in which S_t was formed
+      int on[2] = {0, 0};     // items in which O_t was begun
+      // The products P V run one tile behind the scores, across items too: while
+      // the last weights of an item are formed, the next item's scores are. An
+      // item without work only lets the last products through: the softmax warps
+      // take no further item before them, and so none is asked for.
+      bool use[2] = {false, false};    // P_t of the tile before is to be used,
+      bool begin[2] = {false, false};  // begins O_t,
+      bool end[2] = {false, false};    // ends it
+      bool held = false;               // the V tile before is still needed
+      int w = blockIdx.x;
+      while (ok) {
+        const WaItem a(max(w, 0), B, H, rep, S, blocks, window, sinks, lengths);
+        const int tiles = w >= 0 ? a.tiles : 0;
+        bool begun[2] = {false, false};
+        for (int k = 0; k < max(tiles, 1) && ok; ++k) {
+          const bool more = k < tiles;
+          const int j = a.all.tile(k);
+          const int ks = kv % kWaStages, vs = (kv + kWaStages - 1) % kWaStages;
+          const uint64_t k_desc = desc_at(k_desc0, ks * L::kTile), v_desc = desc_at(v_desc0, vs * L::kTile);
+          if (held) ok = warp_wait(&vfull[vs], ((kv - 1) / kWaStages) & 1, status, kStatusTimeoutSmemFull);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (k > 0 && sees(t, jp)) {
-            if (!mbar_wait(&pfull[t], done[t] & 1, status, kStatusTimeoutTmemFull)) {
-              ok = false;
-              break;
+          for (int t = 0; t < 2; ++t) {
+            if (ok && use[t]) {
+              // the first product of an item starts O_t anew: it has to be read
+              if (begin[t]) {
+                ok = warp_wait(&ofree[t], (on[t] & 1) ^ 1, status, kStatusTimeoutTmemEmpty);
+                ++on[t];
+              }
+              ok = ok && warp_wait(&pfull[2 * t], pn[t] & 1, status, kStatusTimeoutTmemFull);
+              tc_fence_after();
+              if (ok) {
+#pragma unroll
+                for (int kk = 0; kk < 6; ++kk)
+                  umma_ts(lead, tmem + 256 + t * 128, tmem + t * 128 + kk * 8, desc_at(v_desc, kk * 2048), IP,
+                          (!begin[t] || kk > 0) ? 1u : 0u);
+                ok = warp_wait(&pfull[2 * t + 1], pn[t] & 1, status, kStatusTimeoutTmemFull);
+                tc_fence_after();
+              }
+              if (ok) {
+#pragma unroll
+                for (int kk = 6; kk < 8; ++kk)
+                  umma_ts(lead, tmem + 256 + t * 128, tmem + t * 128 + kk * 8, desc_at(v_desc, kk * 2048), IP, 1u);
+                if (end[t]) umma_commit_by(lead, &ofull[t]);
+              }
+              ++pn[t];
             }
-            tc_fence_after();
+            use[t] = more && a.sees(t, j);
+            if (use[t]) {
+              begin[t] = !begun[t];
+              end[t] = j == (t ? a.sub1.e : a.sub0.e);
+              begun[t] = true;
+            }
+            if (ok && more) {
+              if (k == 0 && t < a.live) {
+                ok = warp_wait(&qfull[t], sn[t] & 1, status, kStatusTimeoutSmemFull);
+                ++sn[t];
+              }
+              if (ok && t == 0) ok = warp_wait(&kfull[ks], (kv / kWaStages) & 1, status, kStatusTimeoutSmemFull);
+              if (ok && use[t]) {
+                tc_fence_after();
 #pragma unroll
-            for (int kk = 0; kk < 8; ++kk)
-              umma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8,
-                          sdesc_sw128(v_addr + kk * 2048, kWaChunk, 1024), IP,
-                          (done[t] > 0 || kk > 0) ? 1u : 0u);
-            ++done[t];
-            if (jp == (t ? sub1.e : sub0.e)) umma_commit(&ofull[t]);
+                for (int c = 0; c < L::kChunks; ++c)
+#pragma unroll
+                  for (int kk = 0; kk < HeadChunks<HD>::steps(c); ++kk)
+                    umma_ss(lead, tmem + t * 128, desc_at(q_desc, t * L::kTile + c * kWaChunk + kk * 32),
+                            desc_at(k_desc, c * kWaChunk + kk * 32), IS, (c > 0 || kk > 0) ? 1u : 0u);
+                umma_commit_by(lead, &sfull[t]);
+                if (end[t]) umma_commit_by(lead, &qempty[t]);
+              }
+            }
           }
-          if (k < tiles && sees(t, j)) {
-#pragma unroll
-            for (int c = 0; c < L::kChunks; ++c)
-#pragma unroll
-              for (int kk = 0; kk < HeadChunks<HD>::steps(c); ++kk)
-                umma_f16(tmem + t * 128,
-                         sdesc_sw128(q_addr + t * L::kTile + c * kWaChunk + kk * 32, 16, 1024),
-                         sdesc_sw128(k_addr + c * kWaChunk + kk * 32, 16, 1024), IS,
-                         (c > 0 || kk > 0) ? 1u : 0u);
-            umma_commit(&sfull[t]);
+          if (ok && held) umma_commit_by(lead, &vempty[vs]);
+          held = more;
+          if (more) {
+            if (ok) umma_commit_by(lead, &kempty[ks]);
+            ++kv;
           }
         }
-        if (!ok) break;
-        if (k < tiles) umma_commit(&kempty[ks]);
-        if (k > 0) umma_commit(&vempty[vs]);
+        if (w < 0) break;
+        w = queue.next(status, lane);
       }
-      umma_commit(drain);
+      umma_commit_by(lead, drain);
       mbar_wait(drain, 0, nullptr, kStatusTimeoutDrain);
     }
   } else {
-    const int t = (warp - 2) >> 2;
+    reg_inc<kWaRegsSoftmax>();
+    const int t = (warp - 4) >> 2;  // subtile
     const int wq = warp & 3;
     const int r = wq * 32 + lane;  // row of the subtile = TMEM lane
-    const int row = q0 + t * 128 + r;
     const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
     const uint32_t s_t = tmem + t * 128 + lanes, o_t = tmem + 256 + t * 128 + lanes;
-    const TileList& sub = t ? sub1 : sub0;
-    const int mine = t < live ? sub.count() : 0;
-    const int first = q0 + t * 128;
-    float m = -INFINITY, l = 0.f;
+    uint8_t* stage = smem + L::kStage + (warp - 4) * 4096;
+    const f32x2 scale2 = pair2(scale_log2, scale_log2);
     bool ok = true;
-    for (int i = 0; i < mine; ++i) {
-      if (!mbar_wait(&sfull[t], i & 1, status, kStatusTimeoutTmemFull)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      const int k0 = sub.tile(i) * 128;
-      uint32_t v[128];
+    int sn = 0;     // tiles so far: parity of S_t
+    int items = 0;  // live items so far: parity of O_t
+    for (int w = blockIdx.x; w >= 0; w = ok ? queue.next(status, lane) : -1) {
+      const WaItem a(w, B, H, rep, S, blocks, window, sinks, lengths);
+      const TileList& sub = t ? a.sub1 : a.sub0;
+      const int mine = t < a.live ? sub.count() : 0;
+      const int first = a.q0 + t * 128, row = first + r;
+      float m = -INFINITY, l = 0.f;
+      for (int i = 0; i < mine && ok; ++i, ++sn) {
+        ok = warp_wait(&sfull[t], sn & 1, status, kStatusTimeoutTmemFull);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t v[128];
 #pragma unroll
-      for (int c = 0; c < 8; ++c) tmem_ld16(s_t + c * 16, v + c * 16);
-      tmem_wait_ld();
-      // whole tile visible to every row below the length?
-      const bool whole = k0 + 127 <= first && k0 + 128 <= n &&
-                         (first + 127 - k0 < window || k0 + 128 <= sinks);
-      if (!whole) {
-        const int hi = min(row, n - 1) - k0 + 1;       // visible below this column,
-        const int lo = row - k0 - window + 1;          // and from this one
-        const int sk = sinks - k0;                     // or below this one
+        for (int c = 0; c < 4; ++c) tmem_ld32(s_t + c * 32, v + c * 32);
+        tmem_wait_ld();
+        const int k0 = sub.tile(i) * 128;
+        // whole tile visible to every row below the length?
+        const bool whole = k0 + 127 <= first && k0 + 128 <= a.n &&
+                           (first + 127 - k0 < window || k0 + 128 <= sinks);
+        if (!whole) {
+          const int hi = min(row, a.n - 1) - k0 + 1;     // visible below this column,
+          const int lo = row - k0 - window + 1;          // and from this one
+          const int sk = sinks - k0;                     // or below this one
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const uint32_t vis = bits_below(hi - 32 * c) &
-                               (~bits_below(lo - 32 * c) | bits_below(sk - 32 * c));
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!((vis >> e) & 1u)) v[32 * c + e] = 0xff800000u;  // -inf
+          for (int c = 0; c < 4; ++c)
+            mask32(v + 32 * c, bits_below(hi - 32 * c) & (~bits_below(lo - 32 * c) | bits_below(sk - 32 * c)));
         }
-      }
-      float mx = __uint_as_float(v[0]);
+        float mx4[4];
 #pragma unroll
-      for (int e = 1; e < 128; ++e) mx = fmaxf(mx, __uint_as_float(v[e]));
-      mx *= scale_log2;
-      float mnew = m;
-      if (__any_sync(0xffffffffu, mx > m + kWaRescale)) mnew = fmaxf(m, mx);
-      const float alpha = m == -INFINITY ? 0.f : ex2_wa(m - mnew);
-      const float sub_m = mnew == -INFINITY ? 0.f : mnew;  // nothing visible yet: weights 0
-      float rs = 0.f;
+        for (int z = 0; z < 4; ++z) mx4[z] = fmaxf(__uint_as_float(v[z]), __uint_as_float(v[4 + z]));
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t pk[16];
+        for (int e = 8; e < 128; e += 8)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float p0 = ex2_wa(fmaf(__uint_as_float(v[32 * c + 2 * e]), scale_log2, -sub_m));
-          const float p1 = ex2_wa(fmaf(__uint_as_float(v[32 * c + 2 * e + 1]), scale_log2, -sub_m));
-          rs += p0 + p1;
-          pk[e] = pack_bf16x2(p0, p1);
-        }
-        tmem_st16(s_t + c * 16, pk);
-      }
-      l = l * alpha + rs;
-      if (i > 0 && __any_sync(0xffffffffu, mnew != m)) {
+          for (int z = 0; z < 4; ++z)
+            mx4[z] = max3(mx4[z], __uint_as_float(v[e + 2 * z]), __uint_as_float(v[e + 2 * z + 1]));
+        const float mx = max3(fmaxf(mx4[0], mx4[1]), mx4[2], mx4[3]) * scale_log2;
+        float alpha = 1.f;
+        if (__any_sync(0xffffffffu, mx > m + kWaRescale)) {
+          const float mnew = fmaxf(m, mx);
+          alpha = m == -INFINITY ? 0.f : ex2_wa(m - mnew);
+          m = mnew;
+          if (i > 0) {
 #pragma unroll
-        for (int c = 0; c < HD / 16; ++c) {
-          uint32_t ov[16];
-          tmem_ld16(o_t + c * 16, ov);
-          tmem_wait_ld();
+            for (int c = 0; c < HD / 16; ++c) {
+              uint32_t ov[16];
+              tmem_ld16(o_t + c * 16, ov);
+              tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 16; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
-          tmem_st16(o_t + c * 16, ov);
-        }
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&pfull[t]);
-      m = mnew;
-    }
-    if (mine > 0 && ok) ok = mbar_wait(&ofull[t], 0, status, kStatusTimeoutTmemFull);
-    if (ok) {
-      tc_fence_after();
-      const bool in = row < n;  // a row at or past the length: 0, -inf
-      const float inv = in ? 1.0f / l : 0.f;
-      __nv_bfloat16* orow = o + ((static_cast<size_t>(b) * S + row) * H + h) * HD;
-#pragma unroll
-      for (int c = 0; c < HD / 16; ++c) {
-        uint32_t v[16];
-        if (mine > 0) {
-          tmem_ld16(o_t + c * 16, v);
-          tmem_wait_ld();
-        }
-        if (row < S) {
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (in) {
-              w.x = pack_bf16x2(__uint_as_float(v[8 * u]) * inv, __uint_as_float(v[8 * u + 1]) * inv);
-              w.y = pack_bf16x2(__uint_as_float(v[8 * u + 2]) * inv, __uint_as_float(v[8 * u + 3]) * inv);
-              w.z = pack_bf16x2(__uint_as_float(v[8 * u + 4]) * inv, __uint_as_float(v[8 * u + 5]) * inv);
-              w.w = pack_bf16x2(__uint_as_float(v[8 * u + 6]) * inv, __uint_as_float(v[8 * u + 7]) * inv);
+              for (int e = 0; e < 16; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
+              tmem_st16(o_t + c * 16, ov);
             }
-            *reinterpret_cast<uint4*>(orow + c * 16 + u * 8) = w;
           }
         }
+        const float base = m == -INFINITY ? 0.f : m;  // nothing visible yet: weights 0
+        const f32x2 minus2 = pair2(-base, -base);
+        f32x2 sum[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
+          row_weights(v + 32 * c, scale2, minus2, pk, sum);
+          tmem_st16(s_t + c * 16, pk);
+          if (c >= 2) {  // keys 0-95 are enough for the product to start
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&pfull[2 * t + c - 2]);
+          }
+        }
+        float r0, r1;
+        unpair2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), r0, r1);
+        l = l * alpha + (r0 + r1);
       }
-      if (row < S)
-        lse2[(static_cast<size_t>(b) * H + h) * S + row] = in ? m + log2f(l) : -INFINITY;
+      if (ok && mine > 0) ok = warp_wait(&ofull[t], items & 1, status, kStatusTimeoutTmemFull);
+      if (ok) {
+        tc_fence_after();
+        const bool in = row < a.n;  // a row at or past the length: 0, -inf
+        const float inv = in ? 1.0f / l : 0.f;
+        // Through shared memory, so that lanes write along rows: 16 bytes a lane
+        // straight from its own row would touch 32 lines with every store.
+        __nv_bfloat16* oblk = o + ((static_cast<size_t>(a.b) * S + first + wq * 32) * H + a.h) * HD;
+#pragma unroll 1
+        for (int c = 0; c < L::kChunks; ++c) {
+          constexpr int kRest = HD % 64 / 8;  // 16-byte units of a ragged last chunk
+          const bool rest = kRest != 0 && c == L::kChunks - 1;
+          uint32_t y[32];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t v[16];  // past a ragged chunk's end: columns nobody uses
+            if (mine > 0) {
+              tmem_ld16(o_t + c * 64 + e * 16, v);
+              tmem_wait_ld();
+            }
+#pragma unroll
+            for (int z = 0; z < 8; ++z)
+              y[8 * e + z] = in ? pack_bf16x2(__uint_as_float(v[2 * z]) * inv, __uint_as_float(v[2 * z + 1]) * inv) : 0u;
+          }
+          if (mine > 0 && c == L::kChunks - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ofree[t]);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            *reinterpret_cast<uint4*>(stage + lane * 128 + ((e ^ (lane & 7)) << 4)) =
+                make_uint4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
+          __syncwarp();
+          const int units = rest ? kRest : 8, lg = rest ? (kRest == 2 ? 1 : 2) : 3;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            if (e >= units) break;
+            const int rr = (e * 32 + lane) >> lg, u = (e * 32 + lane) & (units - 1);
+            const uint4 x = *reinterpret_cast<const uint4*>(stage + rr * 128 + ((u ^ (rr & 7)) << 4));
+            if (first + wq * 32 + rr < S)
+              *reinterpret_cast<uint4*>(oblk + static_cast<size_t>(rr) * H * HD + c * 64 + u * 8) = x;
+          }
+          __syncwarp();
+        }
+        if (mine > 0) ++items;
+        if (row < S)
+          lse2[(static_cast<size_t>(a.b) * H + a.h) * S + row] = in ? m + log2f(l) : -INFINITY;
+      }
     }
   }
 
@@ -365,9 +531,10 @@ int launch_fwd(const WindowAttnArgs& a, cudaStream_t stream) {
       return 2;
     attr = true;
   }
-  const dim3 grid(a.H, (a.S + 255) / 256, a.B);
-  window_fwd_kernel<HD><<<grid, kWaThreads, L::kSmem, stream>>>(
-      map, a.o, a.lse, a.lengths, a.S, a.H, a.Hkv, std::min(a.window, a.S), std::min(a.sinks, a.S),
+  const int64_t total = static_cast<int64_t>(a.H) * ((a.S + 255) / 256) * a.B;
+  if (total > 0x7fffffff) return 1;
+  window_fwd_kernel<HD><<<static_cast<unsigned>(total), kWaThreads, L::kSmem, stream>>>(
+      map, a.o, a.lse, a.lengths, a.B, a.S, a.H, a.Hkv, std::min(a.window, a.S), std::min(a.sinks, a.S),
       a.scale * kLog2eWa, a.status);
   return cudaGetLastError() == cudaSuccess ? 0 : 2;
 }
@@ -376,7 +543,6 @@ int launch_fwd(const WindowAttnArgs& a, cudaStream_t stream) {
 
 int window_attention_fwd(const WindowAttnArgs& a, cudaStream_t stream) {
   if (a.B < 0 || a.S < 0 || a.H < 1 || a.Hkv < 1 || a.H % a.Hkv || a.window < 1 || a.sinks < 0) return 1;
-  if (a.B > 65535 || a.S > 65535 * 128) return 1;  // the grid's y and z
   if (a.B == 0 || a.S == 0) return 0;
   switch (a.hd) {
     case 64: return launch_fwd<64>(a, stream);

@@ -176,6 +176,23 @@ def test_gpu_padding_is_never_used(cuda, hd, window, sinks):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128])
+def test_gpu_many_more_items_than_sms(cuda, hd):
+    """Each CTA takes many items, empty ones, short ones and full ones in any order."""
+    B, S, H, Hkv = 40, 530, 16, 4
+    g = torch.Generator()
+    g.manual_seed(hd)
+    lengths = torch.randint(0, S + 1, (B,), generator=g).to(torch.int32)
+    lengths[::3] = 0
+    lengths[1::7] = S
+    qkv, dout = inputs(B, S, H, hd, Hkv, cuda, lengths)
+    check(qkv, dout, B, S, H, hd, Hkv, 200, 4, lengths)
+    none = torch.zeros_like(lengths)
+    qkv, dout = inputs(B, S, H, hd, Hkv, cuda, none)
+    check(qkv, dout, B, S, H, hd, Hkv, 200, 4, none)
+
+
+@pytest.mark.gpu
 def test_gpu_strided_rows(cuda):
     """qkv and dout as slices of wider rows give the dense result, bit for bit."""
     B, S, H, hd, Hkv = 2, 200, 4, 64, 2

@@ -149,6 +149,44 @@ __device__ __forceinline__ int next_block_read(const void* answer) {
   return x;
 }
 
+// The items of a CTA: its own block index, then those of blocks that it takes
+// over (next_block_ask), one asked for ahead. Every warp that works on items
+// walks them with one of these.
+struct BlockQueue {
+  void* answer;
+  uint64_t *full, *empty;
+  int seen = 0;
+  // The next item after `w`; -1: none left (or a wait ran out).
+  __device__ __forceinline__ int next(int* status, int lane) {
+    if (!warp_wait(full, seen & 1, status, kStatusTimeoutSmemFull)) return -1;
+    const int w = __shfl_sync(0xffffffffu, next_block_read(answer), 0);
+    ++seen;
+    fence_proxy_async_smem();  // read before the next answer is written over it
+    __syncwarp();
+    if (lane == 0) mbar_arrive(empty);
+    return w;
+  }
+};
+
+// The asking warp: one question at a time, once every role has taken the answer
+// before (`empty` counts the warps that walk the queue).
+__device__ __forceinline__ void ask_blocks(const BlockQueue& q, int* status, int lane) {
+  for (int i = 0;; ++i) {
+    // a wait that ran out: nothing is asked for, and the roles' own waits end
+    if (!warp_wait(q.empty, (i & 1) ^ 1, status, kStatusTimeoutSmemEmpty)) break;
+    if (lane == 0) {
+      mbar_arrive_expect_tx(q.full, 16);
+      next_block_ask(q.answer, q.full);
+    }
+    __syncwarp();
+    if (!warp_wait(q.full, i & 1, status, kStatusTimeoutSmemFull)) {
+      mbar_wait(q.full, i & 1, nullptr, kStatusTimeoutDrain);  // the answer must land
+      break;
+    }
+    if (__shfl_sync(0xffffffffu, next_block_read(q.answer), 0) < 0) break;
+  }
+}
+
 template <int N>
 __device__ __forceinline__ void reg_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
@@ -185,10 +223,34 @@ struct TileList {
   __device__ __forceinline__ int tile(int k) const { return k < ns ? k : w0 + (k - ns); }
 };
 
+// A softmax or epilogue warp's 32 rows x 64 columns (fewer in a ragged last
+// chunk: `units` 16-byte units a row, 8, 4 or 2) as bf16, written along rows
+// through its 4 KB of shared memory: 16 bytes a lane straight from its own row
+// would touch 32 lines with every store. y: the lane's row, `out` row 0 of 32.
+__device__ __forceinline__ void store_rows(const uint32_t* y, uint8_t* stage, __nv_bfloat16* out, int64_t ld,
+                                           int units, int rows, int lane) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    *reinterpret_cast<uint4*>(stage + lane * 128 + ((e ^ (lane & 7)) << 4)) =
+        make_uint4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
+  __syncwarp();
+  const int lg = units == 8 ? 3 : units == 4 ? 2 : 1;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if (e >= units) break;
+    const int r = (e * 32 + lane) >> lg, u = (e * 32 + lane) & (units - 1);
+    const uint4 x = *reinterpret_cast<const uint4*>(stage + r * 128 + ((u ^ (r & 7)) << 4));
+    if (r < rows) *reinterpret_cast<uint4*>(out + r * ld + u * 8) = x;
+  }
+  __syncwarp();
+}
+
 // 64-column chunks of a head and the 16-wide k-steps of chunk c.
 template <int HD>
 struct HeadChunks {
   static constexpr int kCount = (HD + 63) / 64;
+  // 16-byte units of a row of chunk c
+  __device__ static __forceinline__ int units(int c) { return c == kCount - 1 && HD % 64 ? HD % 64 / 8 : 8; }
   __device__ static constexpr int steps(int c) { return (HD - 64 * c >= 64 ? 64 : HD - 64 * c) / 16; }
 };
 

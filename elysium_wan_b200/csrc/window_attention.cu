@@ -87,25 +87,6 @@ struct WaItem {
   }
 };
 
-// The items of a CTA: its own block index, then those of blocks that it takes
-// over (next_block_ask), one asked for ahead. Every warp that works on items
-// walks them with one of these.
-struct WaQueue {
-  const void* answer;
-  uint64_t *full, *empty;
-  int seen = 0;
-  // The next item after `w`; -1: none left (or a wait ran out).
-  __device__ __forceinline__ int next(int* status, int lane) {
-    if (!warp_wait(full, seen & 1, status, kStatusTimeoutSmemFull)) return -1;
-    const int w = __shfl_sync(0xffffffffu, next_block_read(answer), 0);
-    ++seen;
-    fence_proxy_async_smem();  // read before the next answer is written over it
-    __syncwarp();
-    if (lane == 0) mbar_arrive(empty);
-    return w;
-  }
-};
-
 // 32 weights 2^(x scale - base) of a row as bf16 pairs, and their sums in fp32.
 // One pair in four goes to the FMA pipe: a warp's 128 columns take 1250 cycles
 // alone on its scheduler so, 1420 on the special-function unit alone, 1280 with
@@ -188,27 +169,11 @@ __global__ void __launch_bounds__(kWaThreads, 1)
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
-  WaQueue queue{answer, wfull, wempty};
+  BlockQueue queue{answer, wfull, wempty};
   if (warp < 4) {
     reg_dec<kWaRegsIssue>();
     if (warp == 2) {
-      // asks for the next item once every role has taken the one before
-      for (int i = 0;; ++i) {
-        if (!warp_wait(wempty, (i & 1) ^ 1, status, kStatusTimeoutSmemEmpty)) {
-          // nothing is asked for: the roles' own waits end
-          break;
-        }
-        if (lane == 0) {
-          mbar_arrive_expect_tx(wfull, 16);
-          next_block_ask(answer, wfull);
-        }
-        __syncwarp();
-        if (!warp_wait(wfull, i & 1, status, kStatusTimeoutSmemFull)) {
-          mbar_wait(wfull, i & 1, nullptr, kStatusTimeoutDrain);  // the answer must land
-          break;
-        }
-        if (__shfl_sync(0xffffffffu, next_block_read(answer), 0) < 0) break;
-      }
+      ask_blocks(queue, status, lane);
     } else if (warp == 0) {
       bool ok = true;
       int kv = 0, qn[2] = {0, 0}, cleared = 0;  // K / V tiles, Q subtiles, cleared tiles so far
@@ -463,13 +428,9 @@ __global__ void __launch_bounds__(kWaThreads, 1)
         tc_fence_after();
         const bool in = row < a.n;  // a row at or past the length: 0, -inf
         const float inv = in ? 1.0f / l : 0.f;
-        // Through shared memory, so that lanes write along rows: 16 bytes a lane
-        // straight from its own row would touch 32 lines with every store.
         __nv_bfloat16* oblk = o + ((static_cast<size_t>(a.b) * S + first + wq * 32) * H + a.h) * HD;
 #pragma unroll 1
         for (int c = 0; c < L::kChunks; ++c) {
-          constexpr int kRest = HD % 64 / 8;  // 16-byte units of a ragged last chunk
-          const bool rest = kRest != 0 && c == L::kChunks - 1;
           uint32_t y[32];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -487,21 +448,8 @@ __global__ void __launch_bounds__(kWaThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(&ofree[t]);
           }
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            *reinterpret_cast<uint4*>(stage + lane * 128 + ((e ^ (lane & 7)) << 4)) =
-                make_uint4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
-          __syncwarp();
-          const int units = rest ? kRest : 8, lg = rest ? (kRest == 2 ? 1 : 2) : 3;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            if (e >= units) break;
-            const int rr = (e * 32 + lane) >> lg, u = (e * 32 + lane) & (units - 1);
-            const uint4 x = *reinterpret_cast<const uint4*>(stage + rr * 128 + ((u ^ (rr & 7)) << 4));
-            if (first + wq * 32 + rr < S)
-              *reinterpret_cast<uint4*>(oblk + static_cast<size_t>(rr) * H * HD + c * 64 + u * 8) = x;
-          }
-          __syncwarp();
+          store_rows(y, stage, oblk + c * 64, static_cast<int64_t>(H) * HD, HeadChunks<HD>::units(c),
+                     S - first - wq * 32, lane);
         }
         if (mine > 0) ++items;
         if (row < S)

@@ -9,8 +9,11 @@
 // over key tiles for dK and dV, one over query tiles for dQ. S and dP are so
 // formed twice: 7 products for 5.
 //
-// A first kernel writes D and the statistic into rows padded to 128, with lse2 =
-// +inf past the sequence's length: P is then 0 there without a test.
+// A first kernel writes -D and -lse2 into rows padded to 128, -lse2 = -inf past the
+// sequence's length: P is then 0 there without a test.
+//
+// Blocks are taken over as in the forward (cluster launch control), so that one
+// block's loads and first products run under the end of the last.
 //
 // A sinks' key tile is seen by every later query, so its work is split along the
 // queries into parts of a common tile's length. Each part leaves fp32 sums,
@@ -25,124 +28,204 @@
 namespace ewb {
 namespace {
 
-constexpr int kWbThreads = 320;  // producer, MMA issuer, two warpgroups of softmax warps
+// four warpgroups: producer, MMA issuer and the asking warp; epilogue; softmax of
+// each half of a tile's columns
+constexpr int kWbThreads = 512;
+// registers a thread: 80 + 112 + 2 x 160 = 4 x 128, what the launch takes
+constexpr int kWbRegsIssue = 80, kWbRegsEpilogue = 112, kWbRegsSoftmax = 160;
+constexpr int kWbWalkers = 14;  // warps that walk the queue: producer, issuer, 4 epilogue, 8 softmax
 
 // ---------------------------------------------------------------- D and lse2
-// One half warp per (row, head): 16 bytes of o and dO a lane.
+// One half warp per row and four heads: 16 bytes of o and dO a lane and head.
+// Writes -lse2 (-inf past the length, which makes P 0) and -D.
 __global__ void __launch_bounds__(256)
     window_dot_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ dout,
                       int64_t ldo, const float* __restrict__ lse2, const int* __restrict__ lengths,
-                      float* __restrict__ Lp, float* __restrict__ Dp, int S, int Sp, int H, int HD,
+                      float* __restrict__ NL, float* __restrict__ ND, int S, int Sp, int H, int HD,
                       int64_t units) {
+  constexpr int kHeads = 4;
   const int half = threadIdx.x >> 4, l = threadIdx.x & 15;
-  const int64_t u = static_cast<int64_t>(blockIdx.x) * 16 + half;  // (b, s, h), h fastest
-  if (u >= units) return;
-  const int h = static_cast<int>(u % H);
-  const int64_t bs = u / H;
+  const int64_t u = static_cast<int64_t>(blockIdx.x) * 16 + half;  // (b, s, group of heads)
+  if (u >= units) return;  // a half warp leaves as one
+  const int groups = (H + kHeads - 1) / kHeads;
+  const int h0 = static_cast<int>(u % groups) * kHeads;
+  const int64_t bs = u / groups;
   const int s = static_cast<int>(bs % Sp);
   const int64_t b = bs / Sp;
   const int n = lengths != nullptr ? min(max(lengths[b], 0), S) : S;
-  float d = 0.f;
-  if (s < n && 8 * l < HD) {
-    const int64_t row = b * S + s;
-    const uint4 x = *reinterpret_cast<const uint4*>(o + (row * H + h) * HD + 8 * l);
-    const uint4 y = *reinterpret_cast<const uint4*>(dout + row * ldo + static_cast<int64_t>(h) * HD + 8 * l);
-    float f[8], g[8];
-    unpack8_fmt(x, kFmtBf16, 1.0f, f);
-    unpack8_fmt(y, kFmtBf16, 1.0f, g);
+  const bool in = s < n;
+  const int64_t row = b * S + s;
+  uint4 x[kHeads], y[kHeads];
+  float lse[kHeads];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) d = fmaf(f[e], g[e], d);
+  for (int k = 0; k < kHeads; ++k) {
+    x[k] = y[k] = make_uint4(0, 0, 0, 0);
+    lse[k] = INFINITY;
+    if (in && h0 + k < H) {
+      if (8 * l < HD) {
+        x[k] = *reinterpret_cast<const uint4*>(o + (row * H + h0 + k) * HD + 8 * l);
+        y[k] = *reinterpret_cast<const uint4*>(dout + row * ldo + static_cast<int64_t>(h0 + k) * HD + 8 * l);
+      }
+      lse[k] = lse2[(b * H + h0 + k) * S + s];
+    }
   }
 #pragma unroll
-  for (int k = 8; k > 0; k >>= 1) d += __shfl_xor_sync(0xffffffffu, d, k);
-  if (l == 0) {
-    const int64_t at = (b * H + h) * Sp + s;
-    Dp[at] = d;
-    Lp[at] = s < n ? lse2[(b * H + h) * S + s] : INFINITY;
+  for (int k = 0; k < kHeads; ++k) {
+    float f[8], g[8], d = 0.f;
+    unpack8_fmt(x[k], kFmtBf16, 1.0f, f);
+    unpack8_fmt(y[k], kFmtBf16, 1.0f, g);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) d = fmaf(f[e], g[e], d);
+    const uint32_t who = 0xffffu << (threadIdx.x & 16);
+#pragma unroll
+    for (int z = 8; z > 0; z >>= 1) d += __shfl_xor_sync(who, d, z);
+    if (l == 0 && h0 + k < H) {
+      const int64_t at = (b * H + h0 + k) * Sp + s;
+      ND[at] = -d;
+      NL[at] = -lse[k];
+    }
+  }
+}
+
+// Half a row (64 columns) of weights P = 2^(x scale - lse2) in fp32, over the
+// scores in v; nlse: the two -lse2 of each pair of columns, or one for all.
+template <typename F>
+__device__ __forceinline__ void half_weights(uint32_t* v, f32x2 scale2, F nlse) {
+#pragma unroll
+  for (int e = 0; e < 32; ++e) {
+    float p0, p1;
+    unpair2(fma2(pair2(v[2 * e], v[2 * e + 1]), scale2, nlse(e)), p0, p1);
+    v[2 * e] = __float_as_uint(ex2_wa(p0));
+    v[2 * e + 1] = __float_as_uint(ex2_wa(p1));
+  }
+}
+
+// 0 in the places of v whose bit is not set.
+__device__ __forceinline__ void clear32(uint32_t* v, uint32_t bits) {
+#pragma unroll
+  for (int e = 0; e < 32; ++e)
+    if (!((bits >> e) & 1u)) v[e] = 0u;
+}
+
+// Half a row of weights in bf16 to TMEM (32 columns from `at`).
+__device__ __forceinline__ void store_half(uint32_t at, const uint32_t* v) {
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    uint32_t pk[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      pk[e] = pack_bf16x2(__uint_as_float(v[32 * c + 2 * e]), __uint_as_float(v[32 * c + 2 * e + 1]));
+    tmem_st16(at + c * 16, pk);
   }
 }
 
 // ---------------------------------------------------------------- dK, dV
-// A CTA owns 128 keys of one (batch, kv head) and walks (query head of the
-// group, block of 64 queries): S^T = K Q^T and dP^T = V dO^T into one of two
-// TMEM buffers, P^T and dS^T (bf16) into shared memory, then dV += P^T dO and
-// dK += dS^T Q in TMEM. S^T / dP^T of the next pair start before the
-// gradients of this one. TMEM: S^T x2 | dP^T x2 (64 columns each) | dV | dK.
-constexpr uint32_t kKvOffK = 0, kKvOffV = 32768, kKvOffQ = 65536, kKvOffDO = 98304;
-constexpr uint32_t kKvOffL = 131072, kKvOffD = 131584, kKvOffP = 132096 + 1024, kKvOffS = kKvOffP + 32768;
-constexpr uint32_t kKvOffBar = kKvOffS + 32768;
-constexpr int kKvSmem = kKvOffBar + 256 + 1024;
-static_assert(kKvOffP % 1024 == 0 && kKvOffS % 1024 == 0, "swizzled tiles start on 1024 bytes");
-
+// A block is 128 keys of one (batch, kv head), or a part of a sinks' tile; it
+// walks (query head of the group, tile of 128 queries) in order. For each step t
+//   dV += P^T dO of step t - 1;  S^T = K Q^T;  dK += dS^T Q of t - 1;  dP^T = V dO^T
+// in this order, so that the softmax warps form P^T (from S^T) under the second
+// pair of products and dS^T under the first. P^T and dS^T go over the columns
+// of S^T and dP^T as bf16 and are A operands from there, which takes a third of
+// the operand traffic off shared memory. The epilogue warps empty the
+// accumulators while the next block's steps begin.
+// TMEM: S^T | dP^T | dV | dK (128 columns each). Shared memory: K, V, two
+// stages of Q, dO and the statistics.
 struct KvPlan {
   int window, sinks;  // bounded by S
   int sink_tiles;     // key tiles with a sink
   int parts;          // parts of a sinks' tile
-  int span;           // query blocks of a part
+  int span;           // query tiles of a part
+};
+
+template <int HD>
+struct KvLayout {
+  static constexpr int kChunks = HeadChunks<HD>::kCount;
+  static constexpr uint32_t kTile = kChunks * kWaChunk;
+  static constexpr uint32_t kK = 0, kV = kTile, kQ = 2 * kTile, kO = 4 * kTile, kStat = 6 * kTile;
+  static constexpr uint32_t kStage = kStat + 2048, kBar = kStage + 4 * 4096;
+  static constexpr int kSmem = static_cast<int>(kBar) + 512 + 1024;
+};
+
+struct KvItem {
+  int hk, b, kt, part, n, k0, i0, nqs, steps;
+  bool split;
+  __device__ __forceinline__ KvItem(int w, const KvPlan& plan, int B, int S, int Hkv, int rep, const int* lengths) {
+    hk = w % Hkv;
+    w /= Hkv;
+    b = w % B;
+    const int u = w / B, su = plan.sink_tiles * plan.parts;
+    kt = u < su ? u / plan.parts : u - su + plan.sink_tiles;  // earliest keys first
+    part = u < su ? u % plan.parts : 0;
+    split = u < su && plan.parts > 1;
+    n = lengths != nullptr ? min(max(lengths[b], 0), S) : S;
+    n = __shfl_sync(0xffffffffu, n, 0);
+    k0 = kt * 128;
+    // query tiles that see a key of this tile, this part's share of them
+    i0 = kt;
+    int i1 = 0;
+    if (k0 < n) {
+      const int last = k0 < plan.sinks ? n : min(n, k0 + 127 + plan.window);
+      i1 = (last + 127) >> 7;
+      if (split) {
+        i0 += part * plan.span;
+        i1 = min(i1, i0 + plan.span);
+      }
+    }
+    nqs = max(0, i1 - i0);
+    steps = rep * nqs;
+  }
 };
 
 template <int HD>
 __global__ void __launch_bounds__(kWbThreads, 1)
-    window_dkdv_kernel(const __grid_constant__ CUtensorMap map_kv,
-                       const __grid_constant__ CUtensorMap map_q,
-                       const __grid_constant__ CUtensorMap map_do, const float* __restrict__ Lp,
-                       const float* __restrict__ Dp, const int* __restrict__ lengths,
-                       __nv_bfloat16* __restrict__ dqkv, float* __restrict__ part_ws, int S, int Sp,
-                       int H, int Hkv, KvPlan plan, float scale_log2, float scale, int* status) {
+    window_dkdv_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap map_do,
+                       const float* __restrict__ NL, const float* __restrict__ ND,
+                       const int* __restrict__ lengths, __nv_bfloat16* __restrict__ dqkv,
+                       float* __restrict__ part_ws, int B, int S, int Sp, int H, int Hkv, KvPlan plan,
+                       float scale_log2, float scale, int* status) {
+  using L = KvLayout<HD>;
   using C = HeadChunks<HD>;
-  constexpr uint32_t kTile = C::kCount * kWaChunk;  // 128 rows
-  constexpr uint32_t kBlk = C::kCount * 8192;       // 64 rows
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kKvOffBar);
-  uint64_t* kvfull = bars;
-  uint64_t* qfull = bars + 1;  // [2]
-  uint64_t* done = bars + 3;   // [2]  gradient MMAs of a pair finished (stage and P/dS free)
-  uint64_t* sfull = bars + 5;  // [2]
-  uint64_t* sfree = bars + 7;  // [2]
-  uint64_t* pfull = bars + 9;  // [2]
-  uint64_t* fin = bars + 11;
-  uint64_t* drain = bars + 12;
-  uint64_t* landed = bars + 13;  // a query block that the producer clears
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
+  uint64_t* kfull = bars;
+  uint64_t* kempty = bars + 1;
+  uint64_t* vfull = bars + 2;
+  uint64_t* vempty = bars + 3;
+  uint64_t* qfull = bars + 4;   // [2] Q and the statistics
+  uint64_t* qempty = bars + 6;  // [2]
+  uint64_t* gfull = bars + 8;   // [2] dO
+  uint64_t* gempty = bars + 10; // [2]
+  uint64_t* sfull = bars + 12;
+  uint64_t* pfull = bars + 13;
+  uint64_t* dpfull = bars + 14;
+  uint64_t* dsfull = bars + 15;
+  uint64_t* accfull = bars + 16;
+  uint64_t* accfree = bars + 17;
+  uint64_t* landed = bars + 18;  // a query tile that the producer clears
+  uint64_t* drain = bars + 19;
+  uint64_t* wfull = bars + 20;
+  uint64_t* wempty = bars + 21;
+  uint64_t* answer = bars + 22;  // [2], 16-byte aligned
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
 
-  const int hk = blockIdx.x, bz = blockIdx.z;
-  const int u = blockIdx.y, su = plan.sink_tiles * plan.parts;
-  const int kt = u < su ? u / plan.parts : u - su + plan.sink_tiles;  // earliest keys first
-  const int part = u < su ? u % plan.parts : 0;
-  const bool split = u < su && plan.parts > 1;
-  const int n = lengths != nullptr ? min(max(lengths[bz], 0), S) : S;
-  const int k0 = kt * 128, rep = H / Hkv;
-  // query blocks that see a key of this tile, this part's share of them
-  int i0 = 2 * kt, i1 = 0;
-  if (k0 < n) {
-    const int last = k0 < plan.sinks ? n : min(n, k0 + 127 + plan.window);
-    i1 = (last + 63) / 64;
-    if (split) {
-      i0 += part * plan.span;
-      i1 = min(i1, i0 + plan.span);
-    }
-  }
-  const int nqs = max(0, i1 - i0);
-  const int steps = rep * nqs;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int rep = H / Hkv;
   if (warp == 0 && lane == 0) {
-    mbar_init(kvfull, 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&qfull[i], 1);
-      mbar_init(&done[i], 1);
-      mbar_init(&sfull[i], 1);
-      mbar_init(&sfree[i], 8);
-      mbar_init(&pfull[i], 8);
-    }
-    mbar_init(fin, 1);
-    mbar_init(drain, 1);
+    for (int i = 0; i < 12; ++i) mbar_init(&bars[i], 1);
+    mbar_init(sfull, 1);
+    mbar_init(pfull, 8);
+    mbar_init(dpfull, 1);
+    mbar_init(dsfull, 8);
+    mbar_init(accfull, 1);
+    mbar_init(accfree, 4);
     mbar_init(landed, 1);
+    mbar_init(drain, 1);
+    mbar_init(wfull, 1);
+    mbar_init(wempty, kWbWalkers);
     fence_mbar_init();
-    tma_prefetch_desc(&map_kv);
-    tma_prefetch_desc(&map_q);
+    tma_prefetch_desc(&map);
     tma_prefetch_desc(&map_do);
   }
   if (warp == 1) {
@@ -152,226 +235,336 @@ __global__ void __launch_bounds__(kWbThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  BlockQueue queue{answer, wfull, wempty};
 
-  if (warp == 0) {
-    const int clear = (n < S && (n & 63)) ? n >> 6 : -1;  // the block that holds row n
-    bool ok = true;
-    int issued = 0, cleared = 0;
-    if (lane == 0 && steps > 0) {
-      mbar_arrive_expect_tx(kvfull, 2 * kTile);
-      for (int c = 0; c < C::kCount; ++c) {
-        tma_load_3d(smem + kKvOffK + c * kWaChunk, &map_kv, kvfull, (H + hk) * HD + c * 64, k0, bz, status);
-        tma_load_3d(smem + kKvOffV + c * kWaChunk, &map_kv, kvfull, (H + Hkv + hk) * HD + c * 64, k0, bz,
-                    status);
-      }
-    }
-    for (int t = 0; t < steps && ok; ++t) {
-      const int sb = t & 1;
-      const int h = hk * rep + t / nqs, i = i0 + t % nqs;
-      uint8_t* sq = smem + kKvOffQ + sb * 16384;
-      uint8_t* so = smem + kKvOffDO + sb * 16384;
-      uint64_t* bar = i == clear ? landed : &qfull[sb];
-      if (lane == 0) {
-        ok = mbar_wait(&done[sb], ((t >> 1) & 1) ^ 1, status, kStatusTimeoutSmemEmpty);
-        if (ok) {
-          mbar_arrive_expect_tx(bar, 2 * kBlk + 512);
-          for (int c = 0; c < C::kCount; ++c) {
-            tma_load_3d(sq + c * 8192, &map_q, bar, h * HD + c * 64, i * 64, bz, status);
-            tma_load_3d(so + c * 8192, &map_do, bar, h * HD + c * 64, i * 64, bz, status);
+  if (warp < 4) {
+    reg_dec<kWbRegsIssue>();
+    if (warp == 2) {
+      ask_blocks(queue, status, lane);
+    } else if (warp == 0) {
+      bool ok = true;
+      int items = 0, tn = 0, cleared = 0;
+      int kn = 0, vn = 0;              // K and V tiles issued
+      int qn = 0, gn = 0;              // Q and dO tiles issued on their own barriers
+      int last_cleared = -1;           // the last step whose tiles came over `landed`
+      for (int w = blockIdx.x; w >= 0 && ok; w = ok ? queue.next(status, lane) : -1) {
+        const KvItem a(w, plan, B, S, Hkv, rep, lengths);
+        const int clear = (a.n < S && (a.n & 127)) ? a.n >> 7 : -1;  // the tile that holds row n
+        for (int t = 0; t < a.steps && ok; ++t) {
+          const int s = tn & 1;
+          const uint32_t ph = ((tn >> 1) & 1) ^ 1;
+          const int h = a.hk * rep + t / a.nqs, i = a.i0 + t % a.nqs;
+          const bool patch = i == clear;
+          uint8_t* sq = smem + L::kQ + s * L::kTile;
+          uint8_t* sg = smem + L::kO + s * L::kTile;
+          uint8_t* st = smem + L::kStat + s * 1024;
+          if (t == 0) {
+            ok = warp_wait(kempty, (items & 1) ^ 1, status, kStatusTimeoutSmemEmpty);
+            if (!ok) break;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(kfull, L::kTile);
+              for (int c = 0; c < C::kCount; ++c)
+                tma_load_3d(smem + L::kK + c * kWaChunk, &map, kfull, (H + a.hk) * HD + c * 64, a.k0, a.b, status);
+            }
+            ++kn;
           }
-          const int64_t li = (static_cast<int64_t>(bz) * H + h) * Sp + i * 64;
-          bulk_load(smem + kKvOffL + sb * 256, Lp + li, 256, bar);
-          bulk_load(smem + kKvOffD + sb * 256, Dp + li, 256, bar);
-          issued = t + 1;
+          ok = warp_wait(&qempty[s], ph, status, kStatusTimeoutSmemEmpty);
+          // a cleared step comes whole: its dO stage has to be free as well
+          if (patch) ok = ok && warp_wait(&gempty[s], ph, status, kStatusTimeoutSmemEmpty);
+          if (!ok) break;
+          uint64_t* bar = patch ? landed : &qfull[s];
+          if (lane == 0) {
+            mbar_arrive_expect_tx(bar, (patch ? 2 : 1) * L::kTile + 1024);
+            for (int c = 0; c < C::kCount; ++c)
+              tma_load_3d(sq + c * kWaChunk, &map, bar, h * HD + c * 64, i * 128, a.b, status);
+            const int64_t at = (static_cast<int64_t>(a.b) * H + h) * Sp + i * 128;
+            bulk_load(st, NL + at, 512, bar);
+            bulk_load(st + 512, ND + at, 512, bar);
+          }
+          ++qn;
+          if (t == 0) {
+            ok = warp_wait(vempty, (items & 1) ^ 1, status, kStatusTimeoutSmemEmpty);
+            if (ok) {
+              if (lane == 0) {
+                mbar_arrive_expect_tx(vfull, L::kTile);
+                for (int c = 0; c < C::kCount; ++c)
+                  tma_load_3d(smem + L::kV + c * kWaChunk, &map, vfull, (H + Hkv + a.hk) * HD + c * 64, a.k0, a.b,
+                              status);
+              }
+              ++vn;
+            }
+          }
+          if (!patch) {
+            ok = ok && warp_wait(&gempty[s], ph, status, kStatusTimeoutSmemEmpty);
+            if (!ok) break;
+            bar = &gfull[s];
+            if (lane == 0) mbar_arrive_expect_tx(bar, L::kTile);
+          }
+          if (lane == 0)
+            for (int c = 0; c < C::kCount; ++c)
+              tma_load_3d(sg + c * kWaChunk, &map_do, bar, h * HD + c * 64, i * 128, a.b, status);
+          ++gn;
+          if (patch) {
+            last_cleared = tn;
+            ok = ok && warp_wait(landed, cleared & 1, status, kStatusTimeoutSmemFull);
+            ++cleared;
+            const int r0 = a.n & 127, per = (128 - r0) * 8;
+            if (ok) {
+              for (int k = lane; k < 2 * per * C::kCount; k += 32) {
+                const int c = k / per;
+                uint8_t* base = (c & 1) ? sg : sq;
+                *reinterpret_cast<uint4*>(base + (c >> 1) * kWaChunk + r0 * 128 + (k - c * per) * 16) =
+                    make_uint4(0, 0, 0, 0);
+              }
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                mbar_arrive(&qfull[s]);
+                mbar_arrive(&gfull[s]);
+              }
+            }
+          }
+          ++tn;
         }
+        if (a.steps > 0) ++items;
       }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
-      if (ok && i == clear) {
-        if (!mbar_wait(landed, cleared & 1, status, kStatusTimeoutSmemFull)) ok = false;
-        ok = __all_sync(0xffffffffu, ok);
-        ++cleared;
-        const int r0 = n & 63, w = (64 - r0) * 8;
-        for (int k = lane; k < 2 * w * C::kCount; k += 32) {
-          const int c = k / w;
-          uint8_t* base = (c & 1) ? so : sq;
-          *reinterpret_cast<uint4*>(base + (c >> 1) * 8192 + r0 * 128 + (k - c * w) * 16) = make_uint4(0, 0, 0, 0);
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&qfull[sb]);
-      }
-    }
-    if (lane == 0 && steps > 0) {
-      mbar_wait(kvfull, 0, nullptr, kStatusTimeoutDrain);
-      // a cleared block has landed before it was handed over
-      for (int t = issued - 1; t >= 0 && t >= issued - 2; --t)
-        if (i0 + t % nqs != clear) mbar_wait(&qfull[t & 1], (t >> 1) & 1, nullptr, kStatusTimeoutDrain);
-        else if (!ok) mbar_wait(landed, (cleared + 1) & 1, nullptr, kStatusTimeoutDrain);
-    }
-  } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t IS = idesc_bf16_f32(128, 64, false, false);
+      // Loads already issued must land before this CTA's memory goes away.
+      if (kn > 0) mbar_wait(kfull, (kn - 1) & 1, nullptr, kStatusTimeoutDrain);
+      if (vn > 0) mbar_wait(vfull, (vn - 1) & 1, nullptr, kStatusTimeoutDrain);
+      if (cleared > 0) mbar_wait(landed, (cleared - 1) & 1, nullptr, kStatusTimeoutDrain);
+      for (int t = qn - 1; t >= 0 && t >= qn - 2; --t)
+        if (t != last_cleared) mbar_wait(&qfull[t & 1], (t >> 1) & 1, nullptr, kStatusTimeoutDrain);
+      for (int t = gn - 1; t >= 0 && t >= gn - 2; --t)
+        if (t != last_cleared) mbar_wait(&gfull[t & 1], (t >> 1) & 1, nullptr, kStatusTimeoutDrain);
+    } else if (warp == 1) {
+      const uint32_t lead = elect_lane();
+      constexpr uint32_t IS = idesc_bf16_f32(128, 128, false, false);
       constexpr uint32_t IG = idesc_bf16_f32(128, HD, false, true);
-      const uint32_t k_addr = smem_u32(smem + kKvOffK), v_addr = smem_u32(smem + kKvOffV);
-      bool ok = steps > 0 && mbar_wait(kvfull, 0, status, kStatusTimeoutSmemFull);
-      auto grads = [&](int t) -> bool {
-        const int sb = t & 1;
-        if (!mbar_wait(&pfull[sb], (t >> 1) & 1, status, kStatusTimeoutTmemFull)) return false;
-        tc_fence_after();
-        const uint32_t p_addr = smem_u32(smem + kKvOffP + sb * 16384);
-        const uint32_t s_addr = smem_u32(smem + kKvOffS + sb * 16384);
-        const uint32_t q_addr = smem_u32(smem + kKvOffQ + sb * 16384);
-        const uint32_t o_addr = smem_u32(smem + kKvOffDO + sb * 16384);
+      const uint64_t k_desc = sdesc_sw128(smem_u32(smem + L::kK), 16, 1024);
+      const uint64_t v_desc = sdesc_sw128(smem_u32(smem + L::kV), 16, 1024);
+      // Q and dO as K-major (scores) and MN-major (gradients) operands
+      const uint64_t q_desc = sdesc_sw128(smem_u32(smem + L::kQ), 16, 1024);
+      const uint64_t g_desc = sdesc_sw128(smem_u32(smem + L::kO), 16, 1024);
+      const uint64_t qt_desc = sdesc_sw128(smem_u32(smem + L::kQ), kWaChunk, 1024);
+      const uint64_t gt_desc = sdesc_sw128(smem_u32(smem + L::kO), kWaChunk, 1024);
+      bool ok = true;
+      int items = 0, tn = 0, accs = 0;
+      // the step before: to be finished, the first or last of its block
+      bool held = false, first = false, last = false;
+      int w = blockIdx.x;
+      while (ok) {
+        const KvItem a(max(w, 0), plan, B, S, Hkv, rep, lengths);
+        const int steps = w >= 0 ? a.steps : 0;
+        // a block without work only lets the step before through
+        for (int t = 0; t < max(steps, 1) && ok; ++t) {
+          const bool more = t < steps;
+          const int s = tn & 1, sp = s ^ 1;
+          if (held) {  // dV += P^T dO
+            if (first) {
+              ok = warp_wait(accfree, (accs & 1) ^ 1, status, kStatusTimeoutTmemEmpty);
+              ++accs;
+            }
+            ok = ok && warp_wait(pfull, (tn - 1) & 1, status, kStatusTimeoutTmemFull);
+            tc_fence_after();
+            if (ok) {
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          umma_f16(tmem + 256, sdesc_sw128(p_addr + kk * 32, 16, 1024),
-                   sdesc_sw128(o_addr + kk * 2048, 8192, 1024), IG, (t > 0 || kk > 0) ? 1u : 0u);
-          umma_f16(tmem + 384, sdesc_sw128(s_addr + kk * 32, 16, 1024),
-                   sdesc_sw128(q_addr + kk * 2048, 8192, 1024), IG, (t > 0 || kk > 0) ? 1u : 0u);
-        }
-        umma_commit(&done[sb]);
-        return true;
-      };
-      for (int t = 0; t < steps && ok; ++t) {
-        const int sb = t & 1;
-        const uint32_t ph = (t >> 1) & 1;
-        if (!mbar_wait(&qfull[sb], ph, status, kStatusTimeoutSmemFull) ||
-            !mbar_wait(&sfree[sb], ph ^ 1, status, kStatusTimeoutTmemEmpty)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t q_addr = smem_u32(smem + kKvOffQ + sb * 16384);
-        const uint32_t o_addr = smem_u32(smem + kKvOffDO + sb * 16384);
-#pragma unroll
-        for (int c = 0; c < C::kCount; ++c)
-#pragma unroll
-          for (int kk = 0; kk < C::steps(c); ++kk) {
-            const uint32_t acc = (c > 0 || kk > 0) ? 1u : 0u;
-            umma_f16(tmem + sb * 64, sdesc_sw128(k_addr + c * kWaChunk + kk * 32, 16, 1024),
-                     sdesc_sw128(q_addr + c * 8192 + kk * 32, 16, 1024), IS, acc);
-            umma_f16(tmem + 128 + sb * 64, sdesc_sw128(v_addr + c * kWaChunk + kk * 32, 16, 1024),
-                     sdesc_sw128(o_addr + c * 8192 + kk * 32, 16, 1024), IS, acc);
+              for (int kk = 0; kk < 8; ++kk)
+                umma_ts(lead, tmem + 256, tmem + (kk >> 2) * 64 + (kk & 3) * 8,
+                        desc_at(gt_desc, sp * L::kTile + kk * 2048), IG, (!first || kk > 0) ? 1u : 0u);
+              umma_commit_by(lead, &gempty[sp]);
+            }
           }
-        umma_commit(&sfull[sb]);
-        if (t > 0 && !grads(t - 1)) {
-          ok = false;
-          break;
+          if (ok && more) {  // S^T = K Q^T
+            if (t == 0) ok = warp_wait(kfull, items & 1, status, kStatusTimeoutSmemFull);
+            ok = ok && warp_wait(&qfull[s], (tn >> 1) & 1, status, kStatusTimeoutSmemFull);
+            tc_fence_after();
+            if (ok) {
+#pragma unroll
+              for (int c = 0; c < C::kCount; ++c)
+#pragma unroll
+                for (int kk = 0; kk < C::steps(c); ++kk)
+                  umma_ss(lead, tmem, desc_at(k_desc, c * kWaChunk + kk * 32),
+                          desc_at(q_desc, s * L::kTile + c * kWaChunk + kk * 32), IS, (c > 0 || kk > 0) ? 1u : 0u);
+              umma_commit_by(lead, sfull);
+              if (t == steps - 1) umma_commit_by(lead, kempty);
+            }
+          }
+          if (ok && held) {  // dK += dS^T Q
+            ok = warp_wait(dsfull, (tn - 1) & 1, status, kStatusTimeoutTmemFull);
+            tc_fence_after();
+            if (ok) {
+#pragma unroll
+              for (int kk = 0; kk < 8; ++kk)
+                umma_ts(lead, tmem + 384, tmem + 128 + (kk >> 2) * 64 + (kk & 3) * 8,
+                        desc_at(qt_desc, sp * L::kTile + kk * 2048), IG, (!first || kk > 0) ? 1u : 0u);
+              umma_commit_by(lead, &qempty[sp]);
+              if (last) umma_commit_by(lead, accfull);
+            }
+          }
+          if (ok && more) {  // dP^T = V dO^T
+            if (t == 0) ok = warp_wait(vfull, items & 1, status, kStatusTimeoutSmemFull);
+            ok = ok && warp_wait(&gfull[s], (tn >> 1) & 1, status, kStatusTimeoutSmemFull);
+            tc_fence_after();
+            if (ok) {
+#pragma unroll
+              for (int c = 0; c < C::kCount; ++c)
+#pragma unroll
+                for (int kk = 0; kk < C::steps(c); ++kk)
+                  umma_ss(lead, tmem + 128, desc_at(v_desc, c * kWaChunk + kk * 32),
+                          desc_at(g_desc, s * L::kTile + c * kWaChunk + kk * 32), IS, (c > 0 || kk > 0) ? 1u : 0u);
+              umma_commit_by(lead, dpfull);
+              if (t == steps - 1) umma_commit_by(lead, vempty);
+            }
+          }
+          held = more;
+          first = t == 0;
+          last = t == steps - 1;
+          if (more) ++tn;
         }
+        if (w < 0) break;
+        if (steps > 0) ++items;
+        w = queue.next(status, lane);
       }
-      if (ok && grads(steps - 1)) umma_commit(fin);
-      umma_commit(drain);
+      umma_commit_by(lead, drain);
       mbar_wait(drain, 0, nullptr, kStatusTimeoutDrain);
     }
-  } else {
+  } else if (warp < 8) {
+    // ---- epilogue: dV and dK of a block, one key row a lane
+    reg_dec<kWbRegsEpilogue>();
     const int wq = warp & 3;
-    const int g = (warp - 2) >> 2;  // this warpgroup's half of the 64 query columns
-    const int q0 = g * 32;
-    const int r = wq * 32 + lane;  // key row within the tile = TMEM lane
-    const int kpos = k0 + r;
     const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
+    uint8_t* stage = smem + L::kStage + wq * 4096;
+    const int64_t ldq = static_cast<int64_t>(H + 2 * Hkv) * HD;
     bool ok = true;
-    for (int t = 0; t < steps; ++t) {
-      const int sb = t & 1;
-      const uint32_t ph = (t >> 1) & 1;
-      const int i = i0 + t % nqs;
-      if (!mbar_wait(&sfull[sb], ph, status, kStatusTimeoutTmemFull) ||
-          !mbar_wait(&qfull[sb], ph, status, kStatusTimeoutSmemFull)) {
-        ok = false;
-        break;
+    int items = 0;
+    for (int w = blockIdx.x; w >= 0 && ok; w = ok ? queue.next(status, lane) : -1) {
+      const KvItem a(w, plan, B, S, Hkv, rep, lengths);
+      const bool some = a.steps > 0;
+      if (some) {
+        ok = warp_wait(accfull, items & 1, status, kStatusTimeoutTmemFull);
+        if (!ok) break;
+        ++items;
+        tc_fence_after();
       }
-      tc_fence_after();
-      uint32_t sv[32], pv[32];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        tmem_ld16(tmem + sb * 64 + q0 + lanes + c * 16, sv + c * 16);
-        tmem_ld16(tmem + 128 + sb * 64 + q0 + lanes + c * 16, pv + c * 16);
-      }
-      tmem_wait_ld();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sfree[sb]);
-      // P^T / dS^T buffer sb was read by the gradients of pair t - 2.
-      if (!mbar_wait(&done[sb], ph ^ 1, status, kStatusTimeoutSmemEmpty)) {
-        ok = false;
-        break;
-      }
-      // queries of this half that see key kpos: from kpos on, below kpos + window
-      uint32_t vis = 0xffffffffu;
-      const bool whole = i * 64 >= k0 + 127 && k0 + 128 <= n &&
-                         (i * 64 + 63 - k0 < plan.window || k0 + 128 <= plan.sinks);
-      if (!whole) {
-        const int c0 = i * 64 + q0;
-        vis = kpos < n ? ~bits_below(kpos - c0) : 0u;
-        if (kpos >= plan.sinks) vis &= bits_below(kpos + plan.window - c0);
-      }
-      const float* Ls = reinterpret_cast<const float*>(smem + kKvOffL + sb * 256) + q0;
-      const float* Ds = reinterpret_cast<const float*>(smem + kKvOffD + sb * 256) + q0;
-      uint8_t* prow = smem + kKvOffP + sb * 16384 + r * 128;
-      uint8_t* srow = smem + kKvOffS + sb * 16384 + r * 128;
-#pragma unroll
-      for (int u4 = 0; u4 < 4; ++u4) {
-        const int u8 = g * 4 + u4;  // 16-byte unit of the 64-query row
-        uint32_t pk[4], dk[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float pp[2], dd[2];
-#pragma unroll
-          for (int z = 0; z < 2; ++z) {
-            const int q = u4 * 8 + 2 * e + z;  // within this half
-            const bool see = (vis >> q) & 1u;
-            const float p = ex2_wa(__uint_as_float(sv[q]) * scale_log2 - Ls[q]);
-            pp[z] = see ? p : 0.f;
-            dd[z] = see ? p * (__uint_as_float(pv[q]) - Ds[q]) : 0.f;
-          }
-          pk[e] = pack_bf16x2(pp[0], pp[1]);
-          dk[e] = pack_bf16x2(dd[0], dd[1]);
-        }
-        const uint32_t off = static_cast<uint32_t>((u8 ^ (r & 7)) << 4);
-        *reinterpret_cast<uint4*>(prow + off) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-        *reinterpret_cast<uint4*>(srow + off) = make_uint4(dk[0], dk[1], dk[2], dk[3]);
-      }
-      fence_proxy_async_smem();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&pfull[sb]);
-    }
-    if (ok && steps > 0) ok = mbar_wait(fin, 0, status, kStatusTimeoutTmemFull);
-    if (ok) {  // warpgroup 0 writes dV, warpgroup 1 dK
-      tc_fence_after();
-      const int ldq = (H + 2 * Hkv) * HD;
-      __nv_bfloat16* out = dqkv + (static_cast<size_t>(bz) * S + kpos) * ldq + (g ? H + hk : H + Hkv + hk) * HD;
+      const int row0 = a.k0 + wq * 32;
       float* sum = part_ws;
-      if (split)
-        sum += ((((static_cast<size_t>(bz) * Hkv + hk) * plan.sink_tiles + kt) * plan.parts + part) * 128 + r) *
-                   (2 * HD) + g * HD;
-      const float mul = g ? scale : 1.0f;
+      if (a.split)
+        sum += ((((static_cast<size_t>(a.b) * Hkv + a.hk) * plan.sink_tiles + a.kt) * plan.parts + a.part) * 128 +
+                wq * 32 + lane) * (2 * HD);
+#pragma unroll 1
+      for (int z = 0; z < 2; ++z) {  // dV, then dK
+        const float mul = z ? scale : 1.0f;
+        __nv_bfloat16* out = dqkv + (static_cast<int64_t>(a.b) * S + row0) * ldq + (z ? H + a.hk : H + Hkv + a.hk) * HD;
+#pragma unroll 1
+        for (int c = 0; c < C::kCount; ++c) {
+          uint32_t y[32];
 #pragma unroll
-      for (int c = 0; c < HD / 16; ++c) {
-        uint32_t v[16];
-        if (steps > 0) {
-          tmem_ld16(tmem + 256 + g * 128 + lanes + c * 16, v);
-          tmem_wait_ld();
-        } else {
+          for (int e = 0; e < 4; ++e) {
+            uint32_t v[16];
+            if (some) {
+              tmem_ld16(tmem + 256 + z * 128 + lanes + c * 64 + e * 16, v);
+              tmem_wait_ld();
+            } else {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) v[e] = 0u;
+              for (int k = 0; k < 16; ++k) v[k] = 0u;
+            }
+            if (a.split && 2 * e < C::units(c)) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                *reinterpret_cast<uint4*>(sum + z * HD + c * 64 + e * 16 + 4 * k) =
+                    make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              y[8 * e + k] = pack_bf16x2(__uint_as_float(v[2 * k]) * mul, __uint_as_float(v[2 * k + 1]) * mul);
+          }
+          if (some && z == 1 && c == C::kCount - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(accfree);
+          }
+          if (!a.split) store_rows(y, stage, out + c * 64, ldq, C::units(c), S - row0, lane);
         }
-        if (split) {
+      }
+    }
+  } else {
+    reg_inc<kWbRegsSoftmax>();
+    const int wq = warp & 3;
+    const int g = (warp - 8) >> 2;  // half of the 128 query columns
+    const int r = wq * 32 + lane;   // key row within the tile = TMEM lane
+    const uint32_t half = tmem + (static_cast<uint32_t>(wq * 32) << 16) + g * 64;
+    const f32x2 scale2 = pair2(scale_log2, scale_log2);
+    bool ok = true;
+    int tn = 0;
+    for (int w = blockIdx.x; w >= 0 && ok; w = ok ? queue.next(status, lane) : -1) {
+      const KvItem a(w, plan, B, S, Hkv, rep, lengths);
+      const int kpos = a.k0 + r;
+      int i = a.i0;
+      for (int t = 0; t < a.steps; ++t, ++tn) {
+        const int s = tn & 1;
+        ok = warp_wait(sfull, tn & 1, status, kStatusTimeoutTmemFull) &&
+             warp_wait(&qfull[s], (tn >> 1) & 1, status, kStatusTimeoutSmemFull);
+        if (!ok) break;
+        tc_fence_after();
+        const float4* nl = reinterpret_cast<const float4*>(smem + L::kStat + s * 1024) + g * 16;
+        const float4* nd = nl + 32;
+        uint32_t v[64];
+        tmem_ld32(half, v);
+        tmem_ld32(half + 32, v + 32);
+        tmem_wait_ld();
+        half_weights(v, scale2, [&](int e) {
+          const float4 x = nl[e >> 1];
+          return (e & 1) ? pair2(x.z, x.w) : pair2(x.x, x.y);
+        });
+        // queries of this half that see key kpos: from kpos on, below kpos + window
+        uint32_t vis[2] = {0xffffffffu, 0xffffffffu};
+        const bool whole = i * 128 >= a.k0 + 127 && a.k0 + 128 <= a.n &&
+                           (i * 128 + 127 - a.k0 < plan.window || a.k0 + 128 <= plan.sinks);
+        if (!whole) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            *reinterpret_cast<uint4*>(sum + c * 16 + e * 4) = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
-        } else if (kpos < S) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            uint4 w;
-            w.x = pack_bf16x2(__uint_as_float(v[8 * e]) * mul, __uint_as_float(v[8 * e + 1]) * mul);
-            w.y = pack_bf16x2(__uint_as_float(v[8 * e + 2]) * mul, __uint_as_float(v[8 * e + 3]) * mul);
-            w.z = pack_bf16x2(__uint_as_float(v[8 * e + 4]) * mul, __uint_as_float(v[8 * e + 5]) * mul);
-            w.w = pack_bf16x2(__uint_as_float(v[8 * e + 6]) * mul, __uint_as_float(v[8 * e + 7]) * mul);
-            *reinterpret_cast<uint4*>(out + c * 16 + e * 8) = w;
+          for (int c = 0; c < 2; ++c) {
+            const int c0 = i * 128 + g * 64 + c * 32;
+            vis[c] = kpos < a.n ? ~bits_below(kpos - c0) : 0u;
+            if (kpos >= plan.sinks) vis[c] &= bits_below(kpos + plan.window - c0);
+            clear32(v + 32 * c, vis[c]);
           }
         }
+        store_half(half, v);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(pfull);
+        ok = warp_wait(dpfull, tn & 1, status, kStatusTimeoutTmemFull);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t d[32];
+          tmem_ld32(half + 128 + c * 32, d);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float4 x = nd[c * 8 + (e >> 1)];
+            float d0, d1;
+            unpair2(mul2(pair2(v[32 * c + 2 * e], v[32 * c + 2 * e + 1]),
+                         add2(pair2(d[2 * e], d[2 * e + 1]), (e & 1) ? pair2(x.z, x.w) : pair2(x.x, x.y))),
+                    d0, d1);
+            d[2 * e] = __float_as_uint(d0);
+            d[2 * e + 1] = __float_as_uint(d1);
+          }
+          if (!whole) clear32(d, vis[c]);  // dP of a key past the length may be NaN
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            pk[e] = pack_bf16x2(__uint_as_float(d[2 * e]), __uint_as_float(d[2 * e + 1]));
+          tmem_st16(half + 128 + c * 16, pk);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(dsfull);
+        if (++i == a.i0 + a.nqs) i = a.i0;
       }
     }
   }
@@ -418,62 +611,89 @@ __global__ void __launch_bounds__(256)
 }
 
 // ---------------------------------------------------------------- dQ
-// A CTA owns 128 query rows of one (batch, head) and walks the key tiles they
-// see: S = Q K^T and dP = dO V^T into TMEM, dS (bf16) into shared memory, then
-// dQ += dS K in TMEM, issued after S / dP of the next tile. The K tile serves
-// as both a K-major (S) and an MN-major (dQ) operand. TMEM: S | dP | dQ.
-constexpr uint32_t kDqOffQ = 0, kDqOffDO = 32768, kDqOffK = 65536, kDqOffV = 131072;
-constexpr uint32_t kDqOffS = 196608, kDqOffBar = 229376;
-constexpr int kDqSmem = 229376 + 256 + 1024;
+// A block is 128 query rows of one (batch, head); it walks the key tiles they
+// see. For each tile k
+//   dP = dO V^T of tile k - 1;  dQ += dS K of tile k - 2;  S = Q K^T
+// in this order and across blocks: the softmax warps form P of tile k and dS of
+// tile k - 1 under them. dS goes over the columns of its S as bf16 and is an A
+// operand from there; two S buffers take turns. The epilogue warps empty dQ
+// while the next block's tiles begin.
+// TMEM: S x2 | dP | dQ. Shared memory: Q, dO, K x3, V.
+template <int HD>
+struct DqLayout {
+  static constexpr int kChunks = HeadChunks<HD>::kCount;
+  static constexpr uint32_t kTile = kChunks * kWaChunk;
+  static constexpr uint32_t kQ = 0, kO = kTile, kK = 2 * kTile, kV = 5 * kTile;
+  static constexpr uint32_t kStage = 6 * kTile, kBar = kStage + 4 * 4096;
+  static constexpr int kSmem = static_cast<int>(kBar) + 512 + 1024;
+};
+
+struct DqItem {
+  int h, b, hk, q0, n, tiles;
+  TileList list;
+  __device__ __forceinline__ DqItem(int w, int B, int H, int rep, int S, int blocks, int window, int sinks,
+                                    const int* lengths)
+      : list(0, 0, 1, 0) {
+    h = w % H;
+    w /= H;
+    b = w % B;
+    q0 = (blocks - 1 - w / B) * 128;  // the latest rows first: most tiles
+    hk = h / rep;
+    n = lengths != nullptr ? min(max(lengths[b], 0), S) : S;
+    n = __shfl_sync(0xffffffffu, n, 0);
+    list = TileList(q0, min(q0 + 127, max(n, 1) - 1), window, sinks);
+    tiles = q0 < n ? list.count() : 0;
+  }
+};
 
 template <int HD>
 __global__ void __launch_bounds__(kWbThreads, 1)
-    window_dq_kernel(const __grid_constant__ CUtensorMap map_qkv,
-                     const __grid_constant__ CUtensorMap map_do, const float* __restrict__ Lp,
-                     const float* __restrict__ Dp, const int* __restrict__ lengths,
-                     __nv_bfloat16* __restrict__ dqkv, int S, int Sp, int H, int Hkv, int window,
-                     int sinks, float scale_log2, float scale, int* status) {
+    window_dq_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap map_do,
+                     const float* __restrict__ NL, const float* __restrict__ ND, const int* __restrict__ lengths,
+                     __nv_bfloat16* __restrict__ dqkv, int B, int S, int Sp, int H, int Hkv, int window, int sinks,
+                     float scale_log2, float scale, int* status) {
+  using L = DqLayout<HD>;
   using C = HeadChunks<HD>;
-  constexpr uint32_t kTile = C::kCount * kWaChunk;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kDqOffBar);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
   uint64_t* qfull = bars;
-  uint64_t* kfull = bars + 1;   // [2]
-  uint64_t* kempty = bars + 3;  // [2]
-  uint64_t* sfull = bars + 5;
-  uint64_t* sfree = bars + 6;   // S read into registers
-  uint64_t* pfull = bars + 7;
-  uint64_t* dsfree = bars + 8;  // dQ MMA of the previous tile finished
-  uint64_t* drain = bars + 9;
-  uint64_t* dpfree = bars + 10;  // dP read
-  uint64_t* landed = bars + 11;  // the K tile that the producer clears
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 12);
+  uint64_t* qempty = bars + 1;
+  uint64_t* gfull = bars + 2;  // dO
+  uint64_t* gempty = bars + 3;
+  uint64_t* kfull = bars + 4;   // [3]
+  uint64_t* kempty = bars + 7;  // [3]
+  uint64_t* vfull = bars + 10;
+  uint64_t* vempty = bars + 11;
+  uint64_t* sfull = bars + 12;  // [2]
+  uint64_t* dpfull = bars + 14;
+  uint64_t* dpfree = bars + 15;
+  uint64_t* dsfull = bars + 16;  // [2]
+  uint64_t* accfull = bars + 18;
+  uint64_t* accfree = bars + 19;
+  uint64_t* landed = bars + 20;  // a K tile that the producer clears
+  uint64_t* drain = bars + 21;
+  uint64_t* wfull = bars + 22;
+  uint64_t* wempty = bars + 23;
+  uint64_t* answer = bars + 24;  // [2], 16-byte aligned
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 26);
 
-  const int h = blockIdx.x, bz = blockIdx.z;
-  const int hk = h / (H / Hkv);
-  const int q0 = (gridDim.y - 1 - blockIdx.y) * 128;  // the latest rows first: most tiles
-  const int n = lengths != nullptr ? min(max(lengths[bz], 0), S) : S;
-  const TileList list(q0, min(q0 + 127, max(n, 1) - 1), window, sinks);
-  const int tiles = q0 < n ? list.count() : 0;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int rep = H / Hkv, blocks = Sp / 128;
   if (warp == 0 && lane == 0) {
-    mbar_init(qfull, 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&kfull[i], 1);
-      mbar_init(&kempty[i], 1);
-    }
-    mbar_init(sfull, 1);
-    mbar_init(sfree, 8);
+    for (int i = 0; i < 15; ++i) mbar_init(&bars[i], 1);
     mbar_init(dpfree, 8);
-    mbar_init(pfull, 8);
-    mbar_init(dsfree, 1);
-    mbar_init(drain, 1);
+    mbar_init(&dsfull[0], 8);
+    mbar_init(&dsfull[1], 8);
+    mbar_init(accfull, 1);
+    mbar_init(accfree, 4);
     mbar_init(landed, 1);
+    mbar_init(drain, 1);
+    mbar_init(wfull, 1);
+    mbar_init(wempty, kWbWalkers);
     fence_mbar_init();
-    tma_prefetch_desc(&map_qkv);
+    tma_prefetch_desc(&map);
     tma_prefetch_desc(&map_do);
   }
   if (warp == 1) {
@@ -483,222 +703,290 @@ __global__ void __launch_bounds__(kWbThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  BlockQueue queue{answer, wfull, wempty};
 
-  if (warp == 0) {
-    const int clear = (n < S && (n & 127)) ? n >> 7 : -1;
-    bool ok = true;
-    int issued = 0;
-    if (lane == 0 && tiles > 0) {
-      mbar_arrive_expect_tx(qfull, 2 * kTile);
-      for (int c = 0; c < C::kCount; ++c) {
-        tma_load_3d(smem + kDqOffQ + c * kWaChunk, &map_qkv, qfull, h * HD + c * 64, q0, bz, status);
-        tma_load_3d(smem + kDqOffDO + c * kWaChunk, &map_do, qfull, h * HD + c * 64, q0, bz, status);
-      }
-    }
-    for (int k = 0; k < tiles && ok; ++k) {
-      const int sb = k & 1, j = list.tile(k);
-      uint8_t* sk = smem + kDqOffK + sb * 32768;
-      uint64_t* bar = j == clear ? landed : &kfull[sb];
-      if (lane == 0) {
-        ok = mbar_wait(&kempty[sb], ((k >> 1) & 1) ^ 1, status, kStatusTimeoutSmemEmpty);
-        if (ok) {
-          mbar_arrive_expect_tx(bar, 2 * kTile);
-          for (int c = 0; c < C::kCount; ++c) {
-            tma_load_3d(sk + c * kWaChunk, &map_qkv, bar, (H + hk) * HD + c * 64, j * 128, bz, status);
-            tma_load_3d(smem + kDqOffV + sb * 32768 + c * kWaChunk, &map_qkv, bar,
-                        (H + Hkv + hk) * HD + c * 64, j * 128, bz, status);
+  if (warp < 4) {
+    reg_dec<kWbRegsIssue>();
+    if (warp == 2) {
+      ask_blocks(queue, status, lane);
+    } else if (warp == 0) {
+      bool ok = true;
+      int items = 0, kv = 0, vn = 0, gn = 0, qn = 0, cleared = 0, last_cleared = -1;
+      for (int w = blockIdx.x; w >= 0 && ok; w = ok ? queue.next(status, lane) : -1) {
+        const DqItem a(w, B, H, rep, S, blocks, window, sinks, lengths);
+        const int clear = (a.n < S && (a.n & 127)) ? a.n >> 7 : -1;  // the tile that holds row n
+        for (int k = 0; k < a.tiles && ok; ++k) {
+          const int j = a.list.tile(k), s = kv % 3;
+          uint8_t* sk = smem + L::kK + s * L::kTile;
+          if (k == 0) {
+            ok = warp_wait(qempty, (items & 1) ^ 1, status, kStatusTimeoutSmemEmpty);
+            if (!ok) break;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(qfull, L::kTile);
+              for (int c = 0; c < C::kCount; ++c)
+                tma_load_3d(smem + L::kQ + c * kWaChunk, &map, qfull, a.h * HD + c * 64, a.q0, a.b, status);
+            }
+            ++qn;
           }
-          issued = k + 1;
+          ok = warp_wait(&kempty[s], ((kv / 3) & 1) ^ 1, status, kStatusTimeoutSmemEmpty);
+          if (!ok) break;
+          uint64_t* bar = j == clear ? landed : &kfull[s];
+          if (lane == 0) {
+            mbar_arrive_expect_tx(bar, L::kTile);
+            for (int c = 0; c < C::kCount; ++c)
+              tma_load_3d(sk + c * kWaChunk, &map, bar, (H + a.hk) * HD + c * 64, j * 128, a.b, status);
+          }
+          ++kv;
+          if (j == clear) {
+            ok = warp_wait(landed, cleared & 1, status, kStatusTimeoutSmemFull);
+            ++cleared;
+            last_cleared = kv - 1;
+            const int r0 = a.n & 127, per = (128 - r0) * 8;
+            for (int i = lane; i < per * C::kCount; i += 32) {
+              const int c = i / per;
+              *reinterpret_cast<uint4*>(sk + c * kWaChunk + r0 * 128 + (i - c * per) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&kfull[s]);
+          }
+          if (k == 0) {
+            ok = ok && warp_wait(gempty, (items & 1) ^ 1, status, kStatusTimeoutSmemEmpty);
+            if (!ok) break;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(gfull, L::kTile);
+              for (int c = 0; c < C::kCount; ++c)
+                tma_load_3d(smem + L::kO + c * kWaChunk, &map_do, gfull, a.h * HD + c * 64, a.q0, a.b, status);
+            }
+            ++gn;
+          }
+          ok = ok && warp_wait(vempty, (vn & 1) ^ 1, status, kStatusTimeoutSmemEmpty);
+          if (!ok) break;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(vfull, L::kTile);
+            for (int c = 0; c < C::kCount; ++c)
+              tma_load_3d(smem + L::kV + c * kWaChunk, &map, vfull, (H + Hkv + a.hk) * HD + c * 64, j * 128, a.b,
+                          status);
+          }
+          ++vn;
         }
+        if (a.tiles > 0) ++items;
       }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
-      if (ok && j == clear) {
-        if (!mbar_wait(landed, 0, status, kStatusTimeoutSmemFull)) ok = false;
-        ok = __all_sync(0xffffffffu, ok);
-        const int r0 = n & 127, w = (128 - r0) * 8;
-        for (int i = lane; i < w * C::kCount; i += 32) {
-          const int c = i / w;
-          *reinterpret_cast<uint4*>(sk + c * kWaChunk + r0 * 128 + (i - c * w) * 16) = make_uint4(0, 0, 0, 0);
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&kfull[sb]);
-      }
-    }
-    if (lane == 0 && tiles > 0) {
-      mbar_wait(qfull, 0, nullptr, kStatusTimeoutDrain);
-      for (int k = issued - 1; k >= 0 && k >= issued - 2; --k) {
-        if (list.tile(k) == clear) mbar_wait(landed, 0, nullptr, kStatusTimeoutDrain);
-        else mbar_wait(&kfull[k & 1], (k >> 1) & 1, nullptr, kStatusTimeoutDrain);
-      }
-    }
-  } else if (warp == 1) {
-    if (lane == 0) {
+      // Loads already issued must land before this CTA's memory goes away.
+      if (qn > 0) mbar_wait(qfull, (qn - 1) & 1, nullptr, kStatusTimeoutDrain);
+      if (gn > 0) mbar_wait(gfull, (gn - 1) & 1, nullptr, kStatusTimeoutDrain);
+      if (vn > 0) mbar_wait(vfull, (vn - 1) & 1, nullptr, kStatusTimeoutDrain);
+      if (cleared > 0) mbar_wait(landed, (cleared - 1) & 1, nullptr, kStatusTimeoutDrain);
+      for (int k = kv - 1; k >= 0 && k >= kv - 3; --k)
+        if (k != last_cleared) mbar_wait(&kfull[k % 3], (k / 3) & 1, nullptr, kStatusTimeoutDrain);
+    } else if (warp == 1) {
+      const uint32_t lead = elect_lane();
       constexpr uint32_t IS = idesc_bf16_f32(128, 128, false, false);
       constexpr uint32_t IQ = idesc_bf16_f32(128, HD, false, true);
-      const uint32_t q_addr = smem_u32(smem + kDqOffQ), o_addr = smem_u32(smem + kDqOffDO);
-      const uint32_t ds_addr = smem_u32(smem + kDqOffS);
-      bool ok = tiles > 0 && mbar_wait(qfull, 0, status, kStatusTimeoutSmemFull);
-      auto dq = [&](int i) -> bool {
-        const int sb = i & 1;
-        if (!mbar_wait(pfull, i & 1, status, kStatusTimeoutTmemFull)) return false;
-        tc_fence_after();
-        const uint32_t k_addr = smem_u32(smem + kDqOffK + sb * 32768);
+      const uint64_t q_desc = sdesc_sw128(smem_u32(smem + L::kQ), 16, 1024);
+      const uint64_t g_desc = sdesc_sw128(smem_u32(smem + L::kO), 16, 1024);
+      const uint64_t k_desc = sdesc_sw128(smem_u32(smem + L::kK), 16, 1024);
+      const uint64_t kt_desc = sdesc_sw128(smem_u32(smem + L::kK), kWaChunk, 1024);
+      const uint64_t v_desc = sdesc_sw128(smem_u32(smem + L::kV), 16, 1024);
+      bool ok = true;
+      int items = 0, gitems = 0, accs = 0, kv = 0;
+      int dpn = 0, dqn = 0;  // tiles whose dP, whose dQ was issued
+      // the tiles one and two before: there, the first or last of their block
+      bool on1 = false, first1 = false, last1 = false, on2 = false, first2 = false, last2 = false;
+      int w = blockIdx.x;
+      while (ok) {
+        const DqItem a(max(w, 0), B, H, rep, S, blocks, window, sinks, lengths);
+        const int tiles = w >= 0 ? a.tiles : 0;
+        // A block lets both tiles before it through, whatever it has itself: the
+        // epilogue takes no further block before them, and so none is asked for.
+        for (int k = 0; k < max(tiles, 2) && ok; ++k) {
+          const bool more = k < tiles;
+          if (on1) {  // dP = dO V^T
+            if (first1) {
+              ok = warp_wait(gfull, gitems & 1, status, kStatusTimeoutSmemFull);
+              ++gitems;
+            }
+            ok = ok && warp_wait(vfull, dpn & 1, status, kStatusTimeoutSmemFull) &&
+                 warp_wait(dpfree, (dpn & 1) ^ 1, status, kStatusTimeoutTmemEmpty);
+            tc_fence_after();
+            if (ok) {
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          umma_f16(tmem + 256, sdesc_sw128(ds_addr + (kk >> 2) * kWaChunk + (kk & 3) * 32, 16, 1024),
-                   sdesc_sw128(k_addr + kk * 2048, kWaChunk, 1024), IQ, (i > 0 || kk > 0) ? 1u : 0u);
-        umma_commit(&kempty[sb]);
-        umma_commit(dsfree);
-        return true;
-      };
-      for (int k = 0; k < tiles && ok; ++k) {
-        const int sb = k & 1;
-        const uint32_t fr = (k & 1) ^ 1;
-        if (!mbar_wait(&kfull[sb], (k >> 1) & 1, status, kStatusTimeoutSmemFull) ||
-            !mbar_wait(sfree, fr, status, kStatusTimeoutTmemEmpty)) {
-          ok = false;
-          break;
+              for (int c = 0; c < C::kCount; ++c)
+#pragma unroll
+                for (int kk = 0; kk < C::steps(c); ++kk)
+                  umma_ss(lead, tmem + 256, desc_at(g_desc, c * kWaChunk + kk * 32),
+                          desc_at(v_desc, c * kWaChunk + kk * 32), IS, (c > 0 || kk > 0) ? 1u : 0u);
+              umma_commit_by(lead, dpfull);
+              umma_commit_by(lead, vempty);
+              if (last1) umma_commit_by(lead, gempty);
+            }
+            ++dpn;
+          }
+          if (ok && on2) {  // dQ += dS K
+            ok = warp_wait(&dsfull[dqn & 1], (dqn >> 1) & 1, status, kStatusTimeoutTmemFull);
+            if (first2) {
+              ok = ok && warp_wait(accfree, (accs & 1) ^ 1, status, kStatusTimeoutTmemEmpty);
+              ++accs;
+            }
+            tc_fence_after();
+            if (ok) {
+              const uint64_t kd = desc_at(kt_desc, (dqn % 3) * L::kTile);
+#pragma unroll
+              for (int kk = 0; kk < 8; ++kk)
+                umma_ts(lead, tmem + 384, tmem + (dqn & 1) * 128 + (kk >> 2) * 64 + (kk & 3) * 8,
+                        desc_at(kd, kk * 2048), IQ, (!first2 || kk > 0) ? 1u : 0u);
+              umma_commit_by(lead, &kempty[dqn % 3]);
+              if (last2) umma_commit_by(lead, accfull);
+            }
+            ++dqn;
+          }
+          if (ok && more) {  // S = Q K^T
+            if (k == 0) ok = warp_wait(qfull, items & 1, status, kStatusTimeoutSmemFull);
+            ok = ok && warp_wait(&kfull[kv % 3], (kv / 3) & 1, status, kStatusTimeoutSmemFull);
+            tc_fence_after();
+            if (ok) {
+              const uint64_t kd = desc_at(k_desc, (kv % 3) * L::kTile);
+#pragma unroll
+              for (int c = 0; c < C::kCount; ++c)
+#pragma unroll
+                for (int kk = 0; kk < C::steps(c); ++kk)
+                  umma_ss(lead, tmem + (kv & 1) * 128, desc_at(q_desc, c * kWaChunk + kk * 32),
+                          desc_at(kd, c * kWaChunk + kk * 32), IS, (c > 0 || kk > 0) ? 1u : 0u);
+              umma_commit_by(lead, &sfull[kv & 1]);
+              if (k == tiles - 1) umma_commit_by(lead, qempty);
+            }
+            ++kv;
+          }
+          on2 = on1;
+          first2 = first1;
+          last2 = last1;
+          on1 = more;
+          first1 = k == 0;
+          last1 = k == tiles - 1;
         }
-        tc_fence_after();
-        const uint32_t k_addr = smem_u32(smem + kDqOffK + sb * 32768);
-        const uint32_t v_addr = smem_u32(smem + kDqOffV + sb * 32768);
-#pragma unroll
-        for (int c = 0; c < C::kCount; ++c)
-#pragma unroll
-          for (int kk = 0; kk < C::steps(c); ++kk)
-            umma_f16(tmem, sdesc_sw128(q_addr + c * kWaChunk + kk * 32, 16, 1024),
-                     sdesc_sw128(k_addr + c * kWaChunk + kk * 32, 16, 1024), IS,
-                     (c > 0 || kk > 0) ? 1u : 0u);
-        if (!mbar_wait(dpfree, fr, status, kStatusTimeoutTmemEmpty)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-#pragma unroll
-        for (int c = 0; c < C::kCount; ++c)
-#pragma unroll
-          for (int kk = 0; kk < C::steps(c); ++kk)
-            umma_f16(tmem + 128, sdesc_sw128(o_addr + c * kWaChunk + kk * 32, 16, 1024),
-                     sdesc_sw128(v_addr + c * kWaChunk + kk * 32, 16, 1024), IS,
-                     (c > 0 || kk > 0) ? 1u : 0u);
-        umma_commit(sfull);
-        if (k > 0 && !dq(k - 1)) {
-          ok = false;
-          break;
-        }
+        if (w < 0) break;
+        if (tiles > 0) ++items;
+        w = queue.next(status, lane);
       }
-      if (ok) dq(tiles - 1);
-      umma_commit(drain);
+      umma_commit_by(lead, drain);
       mbar_wait(drain, 0, nullptr, kStatusTimeoutDrain);
     }
-  } else {
+  } else if (warp < 8) {
+    // ---- epilogue: dQ of a block, one query row a lane
+    reg_dec<kWbRegsEpilogue>();
     const int wq = warp & 3;
-    const int g = (warp - 2) >> 2;  // this warpgroup's half of the 128 key columns
-    const int c0 = g * 64;
-    const int r = wq * 32 + lane;
-    const int row = q0 + r;
     const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
-    const int64_t li = (static_cast<int64_t>(bz) * H + h) * Sp + row;
-    const float lr = Lp[li], dr = Dp[li];  // padded rows: +inf, 0
+    uint8_t* stage = smem + L::kStage + wq * 4096;
+    const int64_t ldq = static_cast<int64_t>(H + 2 * Hkv) * HD;
     bool ok = true;
-    for (int k = 0; k < tiles; ++k) {
-      if (!mbar_wait(sfull, k & 1, status, kStatusTimeoutTmemFull)) {
-        ok = false;
-        break;
+    int items = 0;
+    for (int w = blockIdx.x; w >= 0 && ok; w = ok ? queue.next(status, lane) : -1) {
+      const DqItem a(w, B, H, rep, S, blocks, window, sinks, lengths);
+      const bool some = a.tiles > 0;
+      if (some) {
+        ok = warp_wait(accfull, items & 1, status, kStatusTimeoutTmemFull);
+        if (!ok) break;
+        ++items;
+        tc_fence_after();
       }
-      tc_fence_after();
-      uint32_t sv[64];
+      const int row0 = a.q0 + wq * 32;
+      __nv_bfloat16* out = dqkv + (static_cast<int64_t>(a.b) * S + row0) * ldq + a.h * HD;
+#pragma unroll 1
+      for (int c = 0; c < C::kCount; ++c) {
+        uint32_t y[32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld16(tmem + lanes + c0 + c * 16, sv + c * 16);
-      tmem_wait_ld();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(sfree);
-      const int k0 = list.tile(k) * 128;
-      uint32_t vis[2] = {0xffffffffu, 0xffffffffu};
-      const bool whole = k0 + 127 <= q0 && q0 + 128 <= n &&
-                         (q0 + 127 - k0 < window || k0 + 128 <= sinks);
-      if (!whole) {
-        const int hi = (row < n ? row : -1) - k0 + 1, lo = row - k0 - window + 1, sk = sinks - k0;
+        for (int e = 0; e < 4; ++e) {
+          uint32_t v[16];
+          if (some) {
+            tmem_ld16(tmem + 384 + lanes + c * 64 + e * 16, v);
+            tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) v[k] = 0u;
+          }
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            y[8 * e + k] = pack_bf16x2(__uint_as_float(v[2 * k]) * scale, __uint_as_float(v[2 * k + 1]) * scale);
+        }
+        if (some && c == C::kCount - 1) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(accfree);
+        }
+        store_rows(y, stage, out + c * 64, ldq, C::units(c), S - row0, lane);
+      }
+    }
+  } else {
+    reg_inc<kWbRegsSoftmax>();
+    const int wq = warp & 3;
+    const int g = (warp - 8) >> 2;  // half of the 128 key columns
+    const int r = wq * 32 + lane;   // query row within the tile = TMEM lane
+    const uint32_t half = tmem + (static_cast<uint32_t>(wq * 32) << 16) + g * 64;
+    const f32x2 scale2 = pair2(scale_log2, scale_log2);
+    bool ok = true;
+    int tn = 0;
+    for (int w = blockIdx.x; w >= 0 && ok; w = ok ? queue.next(status, lane) : -1) {
+      const DqItem a(w, B, H, rep, S, blocks, window, sinks, lengths);
+      const int row = a.q0 + r;
+      const int64_t at = (static_cast<int64_t>(a.b) * H + a.h) * Sp + row;
+      const float nl = NL[at], nd = ND[at];  // padded rows: -inf, 0
+      const f32x2 nl2 = pair2(nl, nl), nd2 = pair2(nd, nd);
+      for (int k = 0; k < a.tiles; ++k, ++tn) {
+        const uint32_t s_t = half + (tn & 1) * 128;
+        ok = warp_wait(&sfull[tn & 1], (tn >> 1) & 1, status, kStatusTimeoutTmemFull);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t v[64];
+        tmem_ld32(s_t, v);
+        tmem_ld32(s_t + 32, v + 32);
+        tmem_wait_ld();
+        half_weights(v, scale2, [&](int) { return nl2; });
+        const int k0 = a.list.tile(k) * 128;
+        uint32_t vis[2] = {0xffffffffu, 0xffffffffu};
+        const bool whole = k0 + 127 <= a.q0 && a.q0 + 128 <= a.n &&
+                           (a.q0 + 127 - k0 < window || k0 + 128 <= sinks);
+        if (!whole) {
+          const int c0 = k0 + g * 64;
+          const int hi = (row < a.n ? row : -1) - c0 + 1, lo = row - c0 - window + 1, sk = sinks - c0;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            vis[c] = bits_below(hi - 32 * c) & (~bits_below(lo - 32 * c) | bits_below(sk - 32 * c));
+            clear32(v + 32 * c, vis[c]);
+          }
+        }
+        ok = warp_wait(dpfull, tn & 1, status, kStatusTimeoutTmemFull);
+        if (!ok) break;
+        tc_fence_after();
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const int at = c0 + 32 * c;
-          vis[c] = bits_below(hi - at) & (~bits_below(lo - at) | bits_below(sk - at));
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 64; ++e) {
-        const float p = ex2_wa(__uint_as_float(sv[e]) * scale_log2 - lr);
-        sv[e] = __float_as_uint((vis[e >> 5] >> (e & 31)) & 1u ? p : 0.f);
-      }
-      // dS buffer: the dQ MMA of the previous tile must be done reading it.
-      if (k > 0 && !mbar_wait(dsfree, (k - 1) & 1, status, kStatusTimeoutSmemEmpty)) {
-        ok = false;
-        break;
-      }
-      uint8_t* srow = smem + kDqOffS + g * kWaChunk + r * 128;  // this half's 64-key chunk
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t dp[32];
-        tmem_ld32(tmem + 128 + lanes + c0 + c * 32, dp);
-        tmem_wait_ld();
-#pragma unroll
-        for (int t4 = 0; t4 < 4; ++t4) {
-          uint32_t pk[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float d[2];
-#pragma unroll
-            for (int z = 0; z < 2; ++z) {
-              const int at = t4 * 8 + 2 * e + z;
-              const float p = __uint_as_float(sv[c * 32 + at]);
-              // dP of a key past the length may be NaN; its weight is 0
-              d[z] = (vis[c] >> at) & 1u ? p * (__uint_as_float(dp[at]) - dr) : 0.f;
-            }
-            pk[e] = pack_bf16x2(d[0], d[1]);
-          }
-          const int unit = c * 4 + t4;
-          *reinterpret_cast<uint4*>(srow + ((unit ^ (r & 7)) << 4)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-        }
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(dpfree);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(pfull);
-    }
-    if (ok && tiles > 0) ok = mbar_wait(dsfree, (tiles - 1) & 1, status, kStatusTimeoutTmemFull);
-    if (ok) {
-      tc_fence_after();
-      __nv_bfloat16* out = dqkv + (static_cast<size_t>(bz) * S + row) * ((H + 2 * Hkv) * HD) + h * HD;
-      // warpgroup g: the g-th half of the head's 16-column groups
-      constexpr int kGroups = HD / 16, kHalf = (kGroups + 1) / 2;
-#pragma unroll
-      for (int k = 0; k < kHalf; ++k) {
-        const int c = g * kHalf + k;
-        if (c >= kGroups) break;
-        uint32_t v[16];
-        if (tiles > 0) {
-          tmem_ld16(tmem + 256 + lanes + c * 16, v);
+          uint32_t d[32];
+          tmem_ld32(half + 256 + c * 32, d);
           tmem_wait_ld();
-        } else {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) v[e] = 0u;
-        }
-        if (row < S) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            uint4 w;
-            w.x = pack_bf16x2(__uint_as_float(v[8 * e]) * scale, __uint_as_float(v[8 * e + 1]) * scale);
-            w.y = pack_bf16x2(__uint_as_float(v[8 * e + 2]) * scale, __uint_as_float(v[8 * e + 3]) * scale);
-            w.z = pack_bf16x2(__uint_as_float(v[8 * e + 4]) * scale, __uint_as_float(v[8 * e + 5]) * scale);
-            w.w = pack_bf16x2(__uint_as_float(v[8 * e + 6]) * scale, __uint_as_float(v[8 * e + 7]) * scale);
-            *reinterpret_cast<uint4*>(out + c * 16 + e * 8) = w;
+          if (c == 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(dpfree);
           }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float d0, d1;
+            unpair2(mul2(pair2(v[32 * c + 2 * e], v[32 * c + 2 * e + 1]), add2(pair2(d[2 * e], d[2 * e + 1]), nd2)),
+                    d0, d1);
+            d[2 * e] = __float_as_uint(d0);
+            d[2 * e + 1] = __float_as_uint(d1);
+          }
+          if (!whole) clear32(d, vis[c]);  // dP of a key past the length may be NaN
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            pk[e] = pack_bf16x2(__uint_as_float(d[2 * e]), __uint_as_float(d[2 * e + 1]));
+          tmem_st16(s_t + c * 16, pk);
         }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&dsfull[tn & 1]);
       }
     }
   }
@@ -718,8 +1006,8 @@ KvPlan make_plan(const WindowAttnArgs& f) {
   p.window = std::min(f.window, f.S);
   p.sinks = std::min(f.sinks, f.S);
   p.sink_tiles = (p.sinks + 127) / 128;
-  p.span = (127 + p.window + 63) / 64;  // the query blocks that a common tile meets
-  const int blocks = (f.S + 63) / 64;
+  p.span = (126 + p.window) / 128 + 1;  // the query tiles that a common tile meets
+  const int blocks = padded(f.S) / 128;
   p.parts = p.sink_tiles > 0 ? std::max(1, (blocks + p.span - 1) / p.span) : 1;
   return p;
 }
@@ -730,39 +1018,41 @@ int launch_bwd(const WindowAttnBwdArgs& a, cudaStream_t stream) {
   const int Sp = padded(f.S);
   const KvPlan plan = make_plan(f);
   const uint64_t width = static_cast<uint64_t>(f.H + 2 * f.Hkv) * HD, owidth = static_cast<uint64_t>(f.H) * HD;
-  CUtensorMap m128, m64, do64, do128;
-  if (!tma_map_bf16_3d(&m128, f.qkv, width, f.S, f.B, f.ldq, 64, 128) ||
-      !tma_map_bf16_3d(&m64, f.qkv, width, f.S, f.B, f.ldq, 64, 64) ||
-      !tma_map_bf16_3d(&do64, a.dout, owidth, f.S, f.B, a.ldo, 64, 64) ||
-      !tma_map_bf16_3d(&do128, a.dout, owidth, f.S, f.B, a.ldo, 64, 128))
+  CUtensorMap m, mdo;
+  if (!tma_map_bf16_3d(&m, f.qkv, width, f.S, f.B, f.ldq, 64, 128) ||
+      !tma_map_bf16_3d(&mdo, a.dout, owidth, f.S, f.B, a.ldo, 64, 128))
     return 1;
   static bool attr = false;
   if (!attr) {
-    if (cudaFuncSetAttribute(window_dkdv_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kKvSmem) !=
+    if (cudaFuncSetAttribute(window_dkdv_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             KvLayout<HD>::kSmem) !=
             cudaSuccess ||
-        cudaFuncSetAttribute(window_dq_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kDqSmem) !=
+        cudaFuncSetAttribute(window_dq_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             DqLayout<HD>::kSmem) !=
             cudaSuccess)
       return 2;
     attr = true;
   }
   const int64_t cells = static_cast<int64_t>(f.B) * f.H * Sp;
-  float* Lp = a.ws;
-  float* Dp = Lp + cells;
-  float* parts = Dp + cells;
-  window_dot_kernel<<<static_cast<unsigned>((cells + 15) / 16), 256, 0, stream>>>(
-      f.o, a.dout, a.ldo, f.lse, f.lengths, Lp, Dp, f.S, Sp, f.H, HD, cells);
+  const int64_t units = plan.sink_tiles * plan.parts + Sp / 128 - plan.sink_tiles;
+  const int64_t kv_blocks = units * f.B * f.Hkv, q_blocks = cells / 128;
+  if (kv_blocks > 0x7fffffff || q_blocks > 0x7fffffff) return 1;
+  float* NL = a.ws;
+  float* ND = NL + cells;
+  float* parts = ND + cells;
+  const int64_t dots = static_cast<int64_t>(f.B) * Sp * ((f.H + 3) / 4);
+  window_dot_kernel<<<static_cast<unsigned>((dots + 15) / 16), 256, 0, stream>>>(
+      f.o, a.dout, a.ldo, f.lse, f.lengths, NL, ND, f.S, Sp, f.H, HD, dots);
   const float sl2 = f.scale * kLog2eWa;
-  const int units = plan.sink_tiles * plan.parts + Sp / 128 - plan.sink_tiles;
-  window_dkdv_kernel<HD><<<dim3(f.Hkv, units, f.B), kWbThreads, kKvSmem, stream>>>(
-      m128, m64, do64, Lp, Dp, f.lengths, a.dqkv, parts, f.S, Sp, f.H, f.Hkv, plan, sl2, f.scale, f.status);
+  window_dkdv_kernel<HD><<<static_cast<unsigned>(kv_blocks), kWbThreads, KvLayout<HD>::kSmem, stream>>>(
+      m, mdo, NL, ND, f.lengths, a.dqkv, parts, f.B, f.S, Sp, f.H, f.Hkv, plan, sl2, f.scale, f.status);
   if (plan.parts > 1) {
     const int64_t t = static_cast<int64_t>(f.B) * f.Hkv * plan.sink_tiles * 128 * (2 * HD / 4);
     window_sinks_kernel<<<static_cast<unsigned>((t + 255) / 256), 256, 0, stream>>>(
         parts, a.dqkv, f.S, f.H, f.Hkv, HD, plan.sink_tiles, plan.parts, f.scale, t);
   }
-  window_dq_kernel<HD><<<dim3(f.H, Sp / 128, f.B), kWbThreads, kDqSmem, stream>>>(
-      m128, do128, Lp, Dp, f.lengths, a.dqkv, f.S, Sp, f.H, f.Hkv, plan.window, plan.sinks, sl2, f.scale,
-      f.status);
+  window_dq_kernel<HD><<<static_cast<unsigned>(q_blocks), kWbThreads, DqLayout<HD>::kSmem, stream>>>(
+      m, mdo, NL, ND, f.lengths, a.dqkv, f.B, f.S, Sp, f.H, f.Hkv, plan.window, plan.sinks, sl2, f.scale, f.status);
   return cudaGetLastError() == cudaSuccess ? 0 : 2;
 }
 
@@ -780,7 +1070,6 @@ int window_attention_bwd_launches(const WindowAttnArgs& f) { return make_plan(f)
 int window_attention_bwd(const WindowAttnBwdArgs& a, cudaStream_t stream) {
   const WindowAttnArgs& f = a.f;
   if (f.B < 0 || f.S < 0 || f.H < 1 || f.Hkv < 1 || f.H % f.Hkv || f.window < 1 || f.sinks < 0) return 1;
-  if (f.B > 65535 || f.S > 65535 * 64) return 1;  // the grid's y and z
   if (f.B == 0 || f.S == 0) return 0;
   switch (f.hd) {
     case 64: return launch_bwd<64>(a, stream);

@@ -193,6 +193,15 @@ def test_gpu_many_more_items_than_sms(cuda, hd):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("S,window", [(100, 30), (257, 1), (130, 500)])
+def test_gpu_many_short_sequences(cuda, S, window):
+    """Blocks of one or two tiles only, several of them a CTA."""
+    B, H, hd, Hkv = 150, 4, 64, 4
+    qkv, dout = inputs(B, S, H, hd, Hkv, cuda)
+    check(qkv, dout, B, S, H, hd, Hkv, window, 2)
+
+
+@pytest.mark.gpu
 def test_gpu_strided_rows(cuda):
     """qkv and dout as slices of wider rows give the dense result, bit for bit."""
     B, S, H, hd, Hkv = 2, 200, 4, 64, 2

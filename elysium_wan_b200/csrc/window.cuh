@@ -223,23 +223,35 @@ struct TileList {
   __device__ __forceinline__ int tile(int k) const { return k < ns ? k : w0 + (k - ns); }
 };
 
+// Four fp32 values of shared memory, the same address in every lane. By its 32-bit
+// address: the aligned base of dynamic shared memory is a generic pointer to the
+// compiler, whose loads are slower.
+__device__ __forceinline__ void lds4(uint32_t addr, f32x2& lo, f32x2& hi) {
+  asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(lo), "=l"(hi) : "r"(addr));
+}
+
 // A softmax or epilogue warp's 32 rows x 64 columns (fewer in a ragged last
 // chunk: `units` 16-byte units a row, 8, 4 or 2) as bf16, written along rows
 // through its 4 KB of shared memory: 16 bytes a lane straight from its own row
 // would touch 32 lines with every store. y: the lane's row, `out` row 0 of 32.
-__device__ __forceinline__ void store_rows(const uint32_t* y, uint8_t* stage, __nv_bfloat16* out, int64_t ld,
+__device__ __forceinline__ void store_rows(const uint32_t* y, uint32_t stage, __nv_bfloat16* out, int64_t ld,
                                            int units, int rows, int lane) {
 #pragma unroll
   for (int e = 0; e < 8; ++e)
-    *reinterpret_cast<uint4*>(stage + lane * 128 + ((e ^ (lane & 7)) << 4)) =
-        make_uint4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(stage + lane * 128 + ((e ^ (lane & 7)) << 4)),
+                 "r"(y[4 * e]), "r"(y[4 * e + 1]), "r"(y[4 * e + 2]), "r"(y[4 * e + 3])
+                 : "memory");
   __syncwarp();
   const int lg = units == 8 ? 3 : units == 4 ? 2 : 1;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     if (e >= units) break;
     const int r = (e * 32 + lane) >> lg, u = (e * 32 + lane) & (units - 1);
-    const uint4 x = *reinterpret_cast<const uint4*>(stage + r * 128 + ((u ^ (r & 7)) << 4));
+    uint4 x;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                 : "r"(stage + r * 128 + ((u ^ (r & 7)) << 4))
+                 : "memory");
     if (r < rows) *reinterpret_cast<uint4*>(out + r * ld + u * 8) = x;
   }
   __syncwarp();

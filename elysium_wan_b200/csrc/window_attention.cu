@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(kWaThreads, 1)
     const int r = wq * 32 + lane;  // row of the subtile = TMEM lane
     const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
     const uint32_t s_t = tmem + t * 128 + lanes, o_t = tmem + 256 + t * 128 + lanes;
-    uint8_t* stage = smem + L::kStage + (warp - 4) * 4096;
+    const uint32_t stage = smem_u32(smem + L::kStage + (warp - 4) * 4096);
     const f32x2 scale2 = pair2(scale_log2, scale_log2);
     bool ok = true;
     int sn = 0;     // tiles so far: parity of S_t

@@ -31,8 +31,8 @@ namespace {
 // four warpgroups: producer, MMA issuer and the asking warp; epilogue; softmax of
 // each half of a tile's columns
 constexpr int kWbThreads = 512;
-// registers a thread: 80 + 112 + 2 x 160 = 4 x 128, what the launch takes
-constexpr int kWbRegsIssue = 80, kWbRegsEpilogue = 112, kWbRegsSoftmax = 160;
+// registers a thread: 64 + 96 + 2 x 176 = 4 x 128, what the launch takes
+constexpr int kWbRegsIssue = 64, kWbRegsEpilogue = 96, kWbRegsSoftmax = 176;
 constexpr int kWbWalkers = 14;  // warps that walk the queue: producer, issuer, 4 epilogue, 8 softmax
 
 // ---------------------------------------------------------------- D and lse2
@@ -87,36 +87,53 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// Half a row (64 columns) of weights P = 2^(x scale - lse2) in fp32, over the
-// scores in v; nlse: the two -lse2 of each pair of columns, or one for all.
+// 32 columns of weights P = 2^(x scale - lse2) in fp32, over the scores in v;
+// nlse(e): the -lse2 of the e-th pair of columns. One pair in four goes to the
+// FMA pipe (see row_weights of the forward).
 template <typename F>
-__device__ __forceinline__ void half_weights(uint32_t* v, f32x2 scale2, F nlse) {
+__device__ __forceinline__ void weights32(uint32_t* v, f32x2 scale2, F nlse) {
 #pragma unroll
-  for (int e = 0; e < 32; ++e) {
+  for (int e = 0; e < 16; ++e) {
+    const f32x2 x = fma2(pair2(v[2 * e], v[2 * e + 1]), scale2, nlse(e));
     float p0, p1;
-    unpair2(fma2(pair2(v[2 * e], v[2 * e + 1]), scale2, nlse(e)), p0, p1);
-    v[2 * e] = __float_as_uint(ex2_wa(p0));
-    v[2 * e + 1] = __float_as_uint(ex2_wa(p1));
+    if (e % 4 == 3) {
+      ex2_poly2(x, p0, p1);
+    } else {
+      unpair2(x, p0, p1);
+      p0 = ex2_wa(p0);
+      p1 = ex2_wa(p1);
+    }
+    v[2 * e] = __float_as_uint(p0);
+    v[2 * e + 1] = __float_as_uint(p1);
   }
+}
+
+// 32 columns of dS = P (dP - D) over dP in d; nd(e): the -D of the e-th pair.
+template <typename F>
+__device__ __forceinline__ void grads32(uint32_t* d, const uint32_t* p, F nd) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    float d0, d1;
+    unpair2(mul2(pair2(p[2 * e], p[2 * e + 1]), add2(pair2(d[2 * e], d[2 * e + 1]), nd(e))), d0, d1);
+    d[2 * e] = __float_as_uint(d0);
+    d[2 * e + 1] = __float_as_uint(d1);
+  }
+}
+
+// 32 columns in bf16 to TMEM (16 columns from `at`).
+__device__ __forceinline__ void store32(uint32_t at, const uint32_t* v) {
+  uint32_t pk[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) pk[e] = pack_bf16x2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
+  tmem_st16(at, pk);
 }
 
 // 0 in the places of v whose bit is not set.
 __device__ __forceinline__ void clear32(uint32_t* v, uint32_t bits) {
+  if (__all_sync(0xffffffffu, bits == 0xffffffffu)) return;
 #pragma unroll
   for (int e = 0; e < 32; ++e)
     if (!((bits >> e) & 1u)) v[e] = 0u;
-}
-
-// Half a row of weights in bf16 to TMEM (32 columns from `at`).
-__device__ __forceinline__ void store_half(uint32_t at, const uint32_t* v) {
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    uint32_t pk[16];
-#pragma unroll
-    for (int e = 0; e < 16; ++e)
-      pk[e] = pack_bf16x2(__uint_as_float(v[32 * c + 2 * e]), __uint_as_float(v[32 * c + 2 * e + 1]));
-    tmem_st16(at + c * 16, pk);
-  }
 }
 
 // ---------------------------------------------------------------- dK, dV
@@ -198,7 +215,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
   uint64_t* gfull = bars + 8;   // [2] dO
   uint64_t* gempty = bars + 10; // [2]
   uint64_t* sfull = bars + 12;
-  uint64_t* pfull = bars + 13;
+  uint64_t* pfull = bars + 13;   // the first 32 queries of each half of P^T; the rest: pfull2
   uint64_t* dpfull = bars + 14;
   uint64_t* dsfull = bars + 15;
   uint64_t* accfull = bars + 16;
@@ -209,6 +226,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
   uint64_t* wempty = bars + 21;
   uint64_t* answer = bars + 22;  // [2], 16-byte aligned
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
+  uint64_t* pfull2 = bars + 25;
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rep = H / Hkv;
@@ -216,6 +234,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
     for (int i = 0; i < 12; ++i) mbar_init(&bars[i], 1);
     mbar_init(sfull, 1);
     mbar_init(pfull, 8);
+    mbar_init(pfull2, 8);
     mbar_init(dpfull, 1);
     mbar_init(dsfull, 8);
     mbar_init(accfull, 1);
@@ -367,13 +386,21 @@ __global__ void __launch_bounds__(kWbThreads, 1)
             }
             ok = ok && warp_wait(pfull, (tn - 1) & 1, status, kStatusTimeoutTmemFull);
             tc_fence_after();
-            if (ok) {
 #pragma unroll
-              for (int kk = 0; kk < 8; ++kk)
-                umma_ts(lead, tmem + 256, tmem + (kk >> 2) * 64 + (kk & 3) * 8,
-                        desc_at(gt_desc, sp * L::kTile + kk * 2048), IG, (!first || kk > 0) ? 1u : 0u);
-              umma_commit_by(lead, &gempty[sp]);
+            for (int z = 0; z < 2; ++z) {
+              if (z == 1) {
+                ok = ok && warp_wait(pfull2, (tn - 1) & 1, status, kStatusTimeoutTmemFull);
+                tc_fence_after();
+              }
+              if (ok) {
+#pragma unroll
+                for (int kk = 0; kk < 8; ++kk)
+                  if (((kk >> 1) & 1) == z)
+                    umma_ts(lead, tmem + 256, tmem + (kk >> 2) * 64 + (kk & 3) * 8,
+                            desc_at(gt_desc, sp * L::kTile + kk * 2048), IG, (!first || kk > 0) ? 1u : 0u);
+              }
             }
+            if (ok) umma_commit_by(lead, &gempty[sp]);
           }
           if (ok && more) {  // S^T = K Q^T
             if (t == 0) ok = warp_wait(kfull, items & 1, status, kStatusTimeoutSmemFull);
@@ -434,7 +461,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
     reg_dec<kWbRegsEpilogue>();
     const int wq = warp & 3;
     const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
-    uint8_t* stage = smem + L::kStage + wq * 4096;
+    const uint32_t stage = smem_u32(smem + L::kStage + wq * 4096);
     const int64_t ldq = static_cast<int64_t>(H + 2 * Hkv) * HD;
     bool ok = true;
     int items = 0;
@@ -507,16 +534,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
              warp_wait(&qfull[s], (tn >> 1) & 1, status, kStatusTimeoutSmemFull);
         if (!ok) break;
         tc_fence_after();
-        const float4* nl = reinterpret_cast<const float4*>(smem + L::kStat + s * 1024) + g * 16;
-        const float4* nd = nl + 32;
-        uint32_t v[64];
-        tmem_ld32(half, v);
-        tmem_ld32(half + 32, v + 32);
-        tmem_wait_ld();
-        half_weights(v, scale2, [&](int e) {
-          const float4 x = nl[e >> 1];
-          return (e & 1) ? pair2(x.z, x.w) : pair2(x.x, x.y);
-        });
+        const uint32_t stat = smem_u32(smem + L::kStat) + s * 1024 + g * 256;
         // queries of this half that see key kpos: from kpos on, below kpos + window
         uint32_t vis[2] = {0xffffffffu, 0xffffffffu};
         const bool whole = i * 128 >= a.k0 + 127 && a.k0 + 128 <= a.n &&
@@ -527,38 +545,39 @@ __global__ void __launch_bounds__(kWbThreads, 1)
             const int c0 = i * 128 + g * 64 + c * 32;
             vis[c] = kpos < a.n ? ~bits_below(kpos - c0) : 0u;
             if (kpos >= plan.sinks) vis[c] &= bits_below(kpos + plan.window - c0);
-            clear32(v + 32 * c, vis[c]);
           }
         }
-        store_half(half, v);
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(pfull);
+        uint32_t v[64];
+        tmem_ld32(half, v);
+        tmem_ld32(half + 32, v + 32);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          f32x2 nl[16];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) lds4(stat + c * 128 + e * 16, nl[2 * e], nl[2 * e + 1]);
+          if (c == 0) tmem_wait_ld();
+          weights32(v + 32 * c, scale2, [&](int e) { return nl[e]; });
+          if (!whole) clear32(v + 32 * c, vis[c]);
+          store32(half + c * 16, v + 32 * c);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(c ? pfull2 : pfull);
+        }
         ok = warp_wait(dpfull, tn & 1, status, kStatusTimeoutTmemFull);
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t d[32];
+          f32x2 nd[16];
           tmem_ld32(half + 128 + c * 32, d);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) lds4(stat + 512 + c * 128 + e * 16, nd[2 * e], nd[2 * e + 1]);
           tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float4 x = nd[c * 8 + (e >> 1)];
-            float d0, d1;
-            unpair2(mul2(pair2(v[32 * c + 2 * e], v[32 * c + 2 * e + 1]),
-                         add2(pair2(d[2 * e], d[2 * e + 1]), (e & 1) ? pair2(x.z, x.w) : pair2(x.x, x.y))),
-                    d0, d1);
-            d[2 * e] = __float_as_uint(d0);
-            d[2 * e + 1] = __float_as_uint(d1);
-          }
+          grads32(d, v + 32 * c, [&](int e) { return nd[e]; });
           if (!whole) clear32(d, vis[c]);  // dP of a key past the length may be NaN
-          uint32_t pk[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            pk[e] = pack_bf16x2(__uint_as_float(d[2 * e]), __uint_as_float(d[2 * e + 1]));
-          tmem_st16(half + 128 + c * 16, pk);
+          store32(half + 128 + c * 16, d);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -877,7 +896,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
     reg_dec<kWbRegsEpilogue>();
     const int wq = warp & 3;
     const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
-    uint8_t* stage = smem + L::kStage + wq * 4096;
+    const uint32_t stage = smem_u32(smem + L::kStage + wq * 4096);
     const int64_t ldq = static_cast<int64_t>(H + 2 * Hkv) * HD;
     bool ok = true;
     int items = 0;
@@ -937,11 +956,6 @@ __global__ void __launch_bounds__(kWbThreads, 1)
         ok = warp_wait(&sfull[tn & 1], (tn >> 1) & 1, status, kStatusTimeoutTmemFull);
         if (!ok) break;
         tc_fence_after();
-        uint32_t v[64];
-        tmem_ld32(s_t, v);
-        tmem_ld32(s_t + 32, v + 32);
-        tmem_wait_ld();
-        half_weights(v, scale2, [&](int) { return nl2; });
         const int k0 = a.list.tile(k) * 128;
         uint32_t vis[2] = {0xffffffffu, 0xffffffffu};
         const bool whole = k0 + 127 <= a.q0 && a.q0 + 128 <= a.n &&
@@ -950,38 +964,33 @@ __global__ void __launch_bounds__(kWbThreads, 1)
           const int c0 = k0 + g * 64;
           const int hi = (row < a.n ? row : -1) - c0 + 1, lo = row - c0 - window + 1, sk = sinks - c0;
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
+          for (int c = 0; c < 2; ++c)
             vis[c] = bits_below(hi - 32 * c) & (~bits_below(lo - 32 * c) | bits_below(sk - 32 * c));
-            clear32(v + 32 * c, vis[c]);
-          }
+        }
+        uint32_t v[64];
+        tmem_ld32(s_t, v);
+        tmem_ld32(s_t + 32, v + 32);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          weights32(v + 32 * c, scale2, [&](int) { return nl2; });
+          if (!whole) clear32(v + 32 * c, vis[c]);
         }
         ok = warp_wait(dpfull, tn & 1, status, kStatusTimeoutTmemFull);
         if (!ok) break;
         tc_fence_after();
+        uint32_t d[64];
+        tmem_ld32(half + 256, d);
+        tmem_ld32(half + 256 + 32, d + 32);
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(dpfree);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          uint32_t d[32];
-          tmem_ld32(half + 256 + c * 32, d);
-          tmem_wait_ld();
-          if (c == 1) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(dpfree);
-          }
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            float d0, d1;
-            unpair2(mul2(pair2(v[32 * c + 2 * e], v[32 * c + 2 * e + 1]), add2(pair2(d[2 * e], d[2 * e + 1]), nd2)),
-                    d0, d1);
-            d[2 * e] = __float_as_uint(d0);
-            d[2 * e + 1] = __float_as_uint(d1);
-          }
-          if (!whole) clear32(d, vis[c]);  // dP of a key past the length may be NaN
-          uint32_t pk[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            pk[e] = pack_bf16x2(__uint_as_float(d[2 * e]), __uint_as_float(d[2 * e + 1]));
-          tmem_st16(s_t + c * 16, pk);
+          grads32(d + 32 * c, v + 32 * c, [&](int) { return nd2; });
+          if (!whole) clear32(d + 32 * c, vis[c]);  // dP of a key past the length may be NaN
+          store32(s_t + c * 16, d + 32 * c);
         }
         tmem_wait_st();
         tc_fence_before();

@@ -11,31 +11,34 @@
 // (x - m) - ln s, so that logits as low as the type goes neither overflow nor
 // drown the rest.
 //
-// Alternatives (up to 32) without a second pass: each thread also keeps where
-// its maximum stood, four neighbouring threads form a quad, and the K-th
-// largest of the quads' maxima bounds the K-th largest logit from below, since
-// K different logits reach it. Only the K quads whose maximum reaches that
-// bound can hold an alternative, so only their share of the row (about K / 128) is read again, out of the
-// L2. A logit and its index make one 64-bit key (greater logit first, then the
-// lower index), so keys are distinct and ranks are counts: no order of arrival
-// shows in the result.
+// Alternatives (up to 32) without a second pass: each thread also keeps which
+// vector its maximum came from, four neighbouring threads form a quad, and the
+// K-th largest of the quads' maxima bounds the K-th largest logit from below,
+// since K different logits reach it. Only quads whose maximum reaches that bound,
+// about K of them, can hold an alternative, so only their share of the row is
+// read again, out of the L2. A logit and its index make one 64-bit key (greater
+// logit first, then the lower index), so keys are distinct and ranks are counts: no
+// order of arrival shows in the result.
 //
-// A cluster of 1, 2, 4 or 8 CTAs shares a row when there are few rows and joins
-// through distributed shared memory.
+// A cluster of 2, 4 or 8 CTAs of 512 threads shares a row when there are few rows
+// and joins through distributed shared memory; with many rows a CTA of 256 threads
+// takes one each, so that one row's end runs under the next one's loads.
 //
 // Rows may start anywhere (an odd vocabulary): vectors are aligned in memory
 // and the two at the ends of the row are read element by element.
+//
+// The gradient is one read and one write. fp32 logits are bound by memory (fp32,
+// 4096 x 50257 forward: 0.9 of the measured copy rate); bf16 ones by the
+// instructions for each logit, hence the packed pairs.
 #include "common.cuh"
 #include "kernels.h"
+#include "pairs.cuh"
 
 #include <algorithm>
 
 namespace ewb {
 namespace {
 
-constexpr int kLpThreads = 512;
-constexpr int kLpWarps = kLpThreads / 32;
-constexpr int kLpQuads = kLpThreads / 4;
 constexpr int kLpTopMax = 32;
 constexpr int kLpCand = 1024;
 constexpr int kLpMaxCluster = 8;
@@ -94,18 +97,20 @@ struct Row {
   __device__ __forceinline__ int vectors() const { return (V + mis + kVE - 1) / kVE; }
   __device__ __forceinline__ int first(int i) const { return i * kVE - mis; }
   // outside the row: -inf, which adds nothing
+  __device__ __forceinline__ void unpack(const uint4& w, float* f) const {
+    if constexpr (sizeof(T) == 4) {
+      f[0] = __uint_as_float(w.x);
+      f[1] = __uint_as_float(w.y);
+      f[2] = __uint_as_float(w.z);
+      f[3] = __uint_as_float(w.w);
+    } else {
+      unpack8_fmt(w, kFmtBf16, 1.0f, f);
+    }
+  }
   __device__ __forceinline__ void load(int i, float* f) const {
     const int j = first(i);
     if (j >= 0 && j + kVE <= V) {
-      const uint4 w = __ldg(reinterpret_cast<const uint4*>(x + j));
-      if constexpr (sizeof(T) == 4) {
-        f[0] = __uint_as_float(w.x);
-        f[1] = __uint_as_float(w.y);
-        f[2] = __uint_as_float(w.z);
-        f[3] = __uint_as_float(w.w);
-      } else {
-        unpack8_fmt(w, kFmtBf16, 1.0f, f);
-      }
+      unpack(__ldg(reinterpret_cast<const uint4*>(x + j)), f);
     } else {
 #pragma unroll
       for (int e = 0; e < kVE; ++e) {
@@ -132,38 +137,67 @@ __device__ __forceinline__ unsigned long long peer_u64(uint32_t a) {
   return v;
 }
 
-// Rank by counting: the keys of list[0..n) with rank < k go to out[rank].
-__device__ __forceinline__ void rank_keys(const unsigned long long* list, int n, int k,
-                                          unsigned long long* out) {
-  for (int i = threadIdx.x; i < n; i += kLpThreads) {
-    const unsigned long long mine = list[i];
-    int r = 0;
-    for (int j = 0; j < n; ++j) r += list[j] > mine ? 1 : 0;
-    if (r < k) out[r] = mine;
-  }
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 
+template <int kThreads>
 struct LpShared {
-  float m[kLpWarps], s[kLpWarps], w[kLpWarps];
-  Sums row;                              // this CTA's sums, read by the cluster
-  unsigned long long quad[kLpQuads];     // the quads' maxima
-  unsigned long long thr;                // lower bound of this CTA's K-th key
+  static constexpr int kWarps = kThreads / 32, kQuads = kThreads / 4;
+  float m[kWarps], s[kWarps], w[kWarps];
+  Sums row;                            // this CTA's sums, read by the cluster
+  unsigned long long quad[kQuads];     // lower bounds of the quads' maxima
+  unsigned long long thr;              // lower bound of this CTA's K-th key
   unsigned long long cand[kLpCand];
-  unsigned long long top[kLpTopMax];     // this CTA's best keys, read by the cluster
+  unsigned long long top[kLpTopMax];   // this CTA's best keys, read by the cluster
   unsigned long long join[kLpTopMax * kLpMaxCluster];
   unsigned long long best;
-  int ncand, ntop;
+  int owner[kQuads];
+  int nowner, ncand, ntop;
 };
 
-template <typename T, bool kTop>
-__global__ void __launch_bounds__(kLpThreads)
+// Adds the logits f (n of them, a maximum cx among them) to a thread's sums.
+template <int n>
+__device__ __forceinline__ void add_logits(Sums& a, const float* f, float cx) {
+  if (cx > a.m) {
+    const float df = fmaxf((a.m - cx) * kLog2eLp, kFloorLp);
+    const float fa = ex2_lp(df);
+    a.w = fa * (a.w + a.s * df);
+    a.s *= fa;
+    a.m = cx;
+  }
+  const float mm = a.m == -INFINITY ? 0.f : a.m;
+  const f32x2 minus2 = pair2(-mm, -mm), log2e2 = pair2(kLog2eLp, kLog2eLp);
+  f32x2 s2[2] = {0ull, 0ull}, w2[2] = {0ull, 0ull};
+#pragma unroll
+  for (int e = 0; e < n; e += 2) {
+    float d0, d1;
+    unpair2(mul2(add2(pair2(f[e], f[e + 1]), minus2), log2e2), d0, d1);
+    d0 = max_nan(d0, kFloorLp);
+    d1 = max_nan(d1, kFloorLp);
+    const f32x2 p = pair2(ex2_lp(d0), ex2_lp(d1));
+    s2[(e >> 1) & 1] = add2(s2[(e >> 1) & 1], p);
+    w2[(e >> 1) & 1] = fma2(p, pair2(d0, d1), w2[(e >> 1) & 1]);
+  }
+  float x, y;
+  unpair2(add2(s2[0], s2[1]), x, y);
+  a.s += x + y;
+  unpair2(add2(w2[0], w2[1]), x, y);
+  a.w += x + y;
+}
+
+template <typename T, bool kTop, int kThreads>
+__global__ void __launch_bounds__(kThreads)
     token_logprobs_kernel(const T* __restrict__ logits, int64_t ld, int V,
                           const int64_t* __restrict__ targets, int top, int cluster,
                           float* __restrict__ logp, float* __restrict__ entropy,
                           float* __restrict__ lse, float* __restrict__ top_logp,
                           int64_t* __restrict__ top_ids, int* status) {
-  __shared__ LpShared sh;
-  constexpr int kVE = Row<T>::kVE;
+  using Sh = LpShared<kThreads>;
+  __shared__ Sh sh;
+  constexpr int kVE = Row<T>::kVE, kWarps = Sh::kWarps, kQuads = Sh::kQuads;
   constexpr int kUnroll = 4;
   const int64_t r = blockIdx.x / cluster;
   const int part = blockIdx.x % cluster;
@@ -181,55 +215,53 @@ __global__ void __launch_bounds__(kLpThreads)
   }
 
   Sums a{-INFINITY, 0.f, 0.f};
-  int bi = max(0, row.first(v0 + tid));  // where this thread's largest logit stands first
+  int bv = v0 + tid;  // the first vector with this thread's largest logit
   const bool any = v0 + tid < v1;
-  for (int i = v0 + tid; i < v1; i += kLpThreads * kUnroll) {
-    float f[kUnroll][kVE];
+  // vectors [1, nv - 1) are whole; the first and the last may not be
+  int i = v0 + tid;
+  for (; i + (kUnroll - 1) * kThreads < v1; i += kThreads * kUnroll) {
+    float f[kUnroll][kVE], cv[kUnroll];
+    if (i > 0 && i + (kUnroll - 1) * kThreads < nv - 1) {
+      uint4 raw[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        raw[u] = __ldg(reinterpret_cast<const uint4*>(row.x + row.first(i + u * kThreads)));
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) row.unpack(raw[u], f[u]);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) row.load(i + u * kThreads, f[u]);
+    }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const int iu = i + u * kLpThreads;
-      if (iu < v1) {
-        row.load(iu, f[u]);
-      } else {
+      cv[u] = fmaxf(f[u][0], f[u][1]);
 #pragma unroll
-        for (int e = 0; e < kVE; ++e) f[u][e] = -INFINITY;
-      }
+      for (int e = 2; e < kVE; e += 2) cv[u] = max3(cv[u], f[u][e], f[u][e + 1]);
     }
-    float cx = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-#pragma unroll
-      for (int e = 0; e < kVE; ++e) cx = fmaxf(cx, f[u][e]);
+    const float cx = fmaxf(max3(cv[0], cv[1], cv[2]), cv[3]);
     if constexpr (kTop) {
       if (cx > a.m) {
 #pragma unroll
         for (int u = kUnroll - 1; u >= 0; --u)
-#pragma unroll
-          for (int e = kVE - 1; e >= 0; --e)
-            if (f[u][e] == cx) bi = row.first(i + u * kLpThreads) + e;
+          if (cv[u] == cx) bv = i + u * kThreads;
       }
     }
-    if (cx > a.m) {
-      const float df = fmaxf((a.m - cx) * kLog2eLp, kFloorLp);
-      const float fa = ex2_lp(df);
-      a.w = fa * (a.w + a.s * df);
-      a.s *= fa;
-      a.m = cx;
-    }
-    const float mm = a.m == -INFINITY ? 0.f : a.m;
+    add_logits<kUnroll * kVE>(a, &f[0][0], cx);
+  }
+  for (; i < v1; i += kThreads) {
+    float f[kVE];
+    row.load(i, f);
+    float cx = f[0];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-#pragma unroll
-      for (int e = 0; e < kVE; ++e) {
-        float d = (f[u][e] - mm) * kLog2eLp;
-        d = d < kFloorLp ? kFloorLp : d;  // keeps a NaN
-        const float p = ex2_lp(d);
-        a.s += p;
-        a.w = fmaf(p, d, a.w);
-      }
+    for (int e = 1; e < kVE; ++e) cx = fmaxf(cx, f[e]);
+    if constexpr (kTop)
+      if (cx > a.m) bv = i;
+    add_logits<kVE>(a, f, cx);
   }
   unsigned long long k = 0ull;
-  if constexpr (kTop) k = any ? make_key(a.m, bi) : 0ull;
+  // The key of the vector's last logit: no greater than the maximum's own, and
+  // less than kVE below it.
+  if constexpr (kTop) k = any ? make_key(a.m, row.first(bv) + kVE - 1) : 0ull;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     Sums b{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o),
@@ -251,41 +283,49 @@ __global__ void __launch_bounds__(kLpThreads)
     if ((lane & 3) == 0) sh.quad[tid >> 2] = k;
     if (tid == 0) {
       sh.thr = 1ull;  // fewer than K quads have logits: every logit counts
-      sh.ncand = 0;
+      sh.ncand = sh.nowner = 0;
     }
   }
   __syncthreads();
-  if (tid == 0) {
-    Sums t{sh.m[0], sh.s[0], sh.w[0]};
-    for (int k = 1; k < kLpWarps; ++k) t = join(t, Sums{sh.m[k], sh.s[k], sh.w[k]});
-    sh.row = t;
+  if (warp == kWarps - 1) {  // the last warp joins the sums, the first ones rank
+    Sums t{-INFINITY, 0.f, 0.f};
+    if (lane < kWarps) t = Sums{sh.m[lane], sh.s[lane], sh.w[lane]};
+#pragma unroll
+    for (int o = kWarps / 2; o > 0; o >>= 1) {
+      Sums b{__shfl_xor_sync(0xffffffffu, t.m, o), __shfl_xor_sync(0xffffffffu, t.s, o),
+             __shfl_xor_sync(0xffffffffu, t.w, o)};
+      t = (lane & o) ? join(b, t) : join(t, b);
+    }
+    if (lane == 0) sh.row = t;
   }
   if constexpr (kTop) {
-    if (tid < kLpQuads) {
+    if (tid < kQuads) {
       const unsigned long long mine = sh.quad[tid];
       int rank = 0;
 #pragma unroll 16
-      for (int j = 0; j < kLpQuads; ++j) rank += sh.quad[j] > mine ? 1 : 0;
+      for (int j = 0; j < kQuads; ++j) rank += sh.quad[j] > mine ? 1 : 0;
       if (rank == top - 1 && mine != 0ull) sh.thr = mine;
     }
     __syncthreads();
     const unsigned long long thr = sh.thr;
-    for (int qw = 0; qw < 8; ++qw) {  // the warp's eight quads, all lanes on one
-      const int q = warp * 8 + qw;
-      const unsigned long long qmax = sh.quad[q];
-      if (qmax < thr || qmax == 0ull) continue;
+    if (tid < kQuads && sh.quad[tid] != 0ull && sh.quad[tid] + (kVE - 1) >= thr)
+      sh.owner[atomicAdd(&sh.nowner, 1)] = tid;
+    __syncthreads();
+    const int owners = sh.nowner;
+    for (int z = warp; z < owners; z += kWarps) {  // all lanes of a warp on one quad
+      const int q = sh.owner[z];
       // lane l: thread q * 4 + l % 4 of rounds l / 4, l / 4 + 8, ...
-      for (int i = v0 + q * 4 + (lane & 3) + (lane >> 2) * kLpThreads; i < v1; i += 8 * kLpThreads) {
+      for (int j = v0 + q * 4 + (lane & 3) + (lane >> 2) * kThreads; j < v1; j += 8 * kThreads) {
         float f[kVE];
-        row.load(i, f);
-        const int j = row.first(i);
+        row.load(j, f);
+        const int at = row.first(j);
 #pragma unroll
         for (int e = 0; e < kVE; ++e) {
-          if (j + e < 0 || j + e >= V) continue;
-          const unsigned long long k = make_key(f[e], j + e);
-          if (k >= thr) {
-            const int at = atomicAdd(&sh.ncand, 1);
-            if (at < kLpCand) sh.cand[at] = k;
+          if (at + e < 0 || at + e >= V) continue;
+          const unsigned long long c = make_key(f[e], at + e);
+          if (c >= thr) {
+            const int n = atomicAdd(&sh.ncand, 1);
+            if (n < kLpCand) sh.cand[n] = c;
           }
         }
       }
@@ -293,7 +333,13 @@ __global__ void __launch_bounds__(kLpThreads)
     __syncthreads();
     const int n = sh.ncand;
     if (n <= kLpCand) {
-      rank_keys(sh.cand, n, top, sh.top);
+      // rank by counting: the candidates of rank < K are the best ones
+      for (int j = tid; j < n; j += kThreads) {
+        const unsigned long long mine = sh.cand[j];
+        int rank = 0;
+        for (int z = 0; z < n; ++z) rank += sh.cand[z] > mine ? 1 : 0;
+        if (rank < top) sh.top[rank] = mine;
+      }
       if (tid == 0) sh.ntop = min(n, top);
     } else {
       // Many logits of few threads at the top (a row of steps): one pass over
@@ -302,19 +348,19 @@ __global__ void __launch_bounds__(kLpThreads)
       for (int t = 0; t < top; ++t) {
         if (tid == 0) sh.best = 0ull;
         __syncthreads();
-        unsigned long long k = 0ull;
-        for (int i = v0 + tid; i < v1; i += kLpThreads) {
+        unsigned long long best = 0ull;
+        for (int j = v0 + tid; j < v1; j += kThreads) {
           float f[kVE];
-          row.load(i, f);
-          const int j = row.first(i);
+          row.load(j, f);
+          const int at = row.first(j);
 #pragma unroll
           for (int e = 0; e < kVE; ++e) {
-            if (j + e < 0 || j + e >= V) continue;
-            const unsigned long long c = make_key(f[e], j + e);
-            if (c < prev && c > k) k = c;
+            if (at + e < 0 || at + e >= V) continue;
+            const unsigned long long c = make_key(f[e], at + e);
+            if (c < prev && c > best) best = c;
           }
         }
-        atomicMax(&sh.best, k);
+        atomicMax(&sh.best, best);
         __syncthreads();
         prev = sh.best;
         if (tid == 0) sh.top[t] = prev;
@@ -336,8 +382,8 @@ __global__ void __launch_bounds__(kLpThreads)
       sh.row = tot;
     }
     if constexpr (kTop) {
-      if (part == 0 && tid < cluster * kLpTopMax) {
-        const int k = tid / kLpTopMax, e = tid % kLpTopMax;
+      if (part == 0 && tid < cluster * top) {
+        const int k = tid / top, e = tid - k * top;
         const int have = peer_s32(peer_smem(smem_u32(&sh.ntop), k));
         sh.join[tid] = e < have ? peer_u64(peer_smem(smem_u32(&sh.top[e]), k)) : 0ull;
       }
@@ -345,7 +391,7 @@ __global__ void __launch_bounds__(kLpThreads)
     cluster_sync_all();  // nobody leaves while its shared memory is read
     if (part != 0) return;
     if constexpr (kTop) {
-      const int n = cluster * kLpTopMax;
+      const int n = cluster * top;  // at most 256: one a thread
       if (tid < n && sh.join[tid] != 0ull) {
         const unsigned long long mine = sh.join[tid];
         int rank = 0;
@@ -387,100 +433,178 @@ __global__ void __launch_bounds__(kLpThreads)
 
 // ---------------------------------------------------------------- gradient
 // d = p (A + B u) + gl [v = t] with u = log2 p, A = -(gl + ge H), B = -ge ln 2.
-// Bound by memory: the logits read and the gradient written once. Rows that
-// are 16-byte aligned on both sides go in vectors of eight; others (an odd
-// vocabulary) one element per lane, whose loads and stores still coalesce.
+// Rows that are 16-byte aligned on both sides go in vectors of eight. Others (an odd
+// vocabulary: every row starts elsewhere) are read in vectors aligned for the
+// logits and written in vectors aligned for the gradient, through shared memory:
+// 4096 x 50257 fp32 to bf16 took 247 us one element a lane, 268 in pairs.
 constexpr int kLgThreads = 256;
+constexpr int kLgChunk = 4096;  // columns of a block
 
-// x - lse first: it is exact to half a unit of the (small) difference.
-__device__ __forceinline__ float lp_grad(float x, float lse, float A, float B) {
-  float u = (x - lse) * kLog2eLp;
-  u = u < kFloorLp ? kFloorLp : u;
-  return ex2_lp(u) * fmaf(B, u, A);
+struct LpRow {
+  f32x2 minus_lse, A, B;
+  float gl;
+  int t;  // -1: none given
+  __device__ __forceinline__ LpRow(int64_t r, int V, const int64_t* targets, const float* lse, const float* entropy,
+                                   const float* g_logp, const float* g_entropy) {
+    const float z = lse[r];
+    const int64_t given = targets != nullptr ? targets[r] : -1;
+    t = given >= 0 && given < V ? static_cast<int>(given) : -1;
+    gl = t >= 0 && g_logp != nullptr ? g_logp[r] : 0.f;
+    const float ge = g_entropy != nullptr ? g_entropy[r] : 0.f;
+    const float a = -(gl + ge * entropy[r]), b = -ge * kLn2Lp;
+    // no finite logit: every p is 0, as an lse of +inf makes it
+    const float minus = z == -INFINITY ? -INFINITY : -z;
+    minus_lse = pair2(minus, minus);
+    A = pair2(a, a);
+    B = pair2(b, b);
+  }
+  // The gradients of n logits from column j on, over the logits in f.
+  // x - lse first: it is exact to half a unit of the (small) difference.
+  template <int n>
+  __device__ __forceinline__ void apply(float* f, int j) const {
+#pragma unroll
+    for (int e = 0; e < n; e += 2) {
+      float u0, u1;
+      unpair2(mul2(add2(pair2(f[e], f[e + 1]), minus_lse), pair2(kLog2eLp, kLog2eLp)), u0, u1);
+      u0 = max_nan(u0, kFloorLp);
+      u1 = max_nan(u1, kFloorLp);
+      unpair2(mul2(pair2(ex2_lp(u0), ex2_lp(u1)), fma2(B, pair2(u0, u1), A)), f[e], f[e + 1]);
+    }
+    if (t >= j && t < j + n) {
+#pragma unroll
+      for (int e = 0; e < n; ++e)
+        if (t == j + e) f[e] += gl;
+    }
+  }
+};
+
+template <typename TG>
+__device__ __forceinline__ TG to_grad(float v) {
+  if constexpr (sizeof(TG) == 4) return v;
+  else return __float2bfloat16_rn(v);
 }
 
-template <typename T, typename TG, bool kVec>
+template <typename T, typename TG>
 __global__ void __launch_bounds__(kLgThreads)
-    token_logprobs_bwd_kernel(const T* __restrict__ logits, int64_t ld, int V,
-                              const int64_t* __restrict__ targets, const float* __restrict__ lse,
-                              const float* __restrict__ entropy, const float* __restrict__ g_logp,
-                              const float* __restrict__ g_entropy, TG* __restrict__ grad,
-                              int64_t ldg, int cols, int64_t rows) {
-  constexpr int kPer = kVec ? 8 : 16;  // elements a thread handles per step
+    token_logprobs_bwd_vec_kernel(const T* __restrict__ logits, int64_t ld, int V,
+                                  const int64_t* __restrict__ targets, const float* __restrict__ lse,
+                                  const float* __restrict__ entropy, const float* __restrict__ g_logp,
+                                  const float* __restrict__ g_entropy, TG* __restrict__ grad,
+                                  int64_t ldg, int cols, int64_t rows) {
+  constexpr int kRounds = kLgChunk / (8 * kLgThreads);
   for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
     const T* x = logits + r * ld;
     TG* g = grad + r * ldg;
-    // no finite logit: every p is 0, as an lse of +inf makes it
-    const float z = lse[r] == -INFINITY ? INFINITY : lse[r];
-    const int64_t t = targets != nullptr ? targets[r] : -1;
-    const bool given = t >= 0 && t < V;
-    const float gl = given && g_logp != nullptr ? g_logp[r] : 0.f;
-    const float ge = g_entropy != nullptr ? g_entropy[r] : 0.f;
-    const float A = -(gl + ge * entropy[r]), B = -ge * kLn2Lp;
-    const int step = gridDim.x * kLgThreads * kPer;
-    for (int j0 = blockIdx.x * kLgThreads * kPer; j0 < cols; j0 += step) {
-      if constexpr (kVec) {
-        const int j = j0 + threadIdx.x * 8;
-        if (j >= cols) continue;
-        float f[8];
-        if (j + 8 <= V) {
-          if constexpr (sizeof(T) == 4) {
-            const uint4 w = __ldcs(reinterpret_cast<const uint4*>(x + j));
-            const uint4 q = __ldcs(reinterpret_cast<const uint4*>(x + j) + 1);
-            const uint32_t u[8] = {w.x, w.y, w.z, w.w, q.x, q.y, q.z, q.w};
+    const LpRow c(r, V, targets, lse, entropy, g_logp, g_entropy);
+    const int j1 = blockIdx.x * kLgChunk + threadIdx.x * 8;
+    float f[kRounds][8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(u[e]);
-          } else {
-            unpack8_fmt(__ldcs(reinterpret_cast<const uint4*>(x + j)), kFmtBf16, 1.0f, f);
-          }
+    for (int k = 0; k < kRounds; ++k) {
+      const int j = j1 + k * kLgThreads * 8;
+      if (j + 8 <= V) {
+        if constexpr (sizeof(T) == 4) {
+          const uint4 w = __ldcs(reinterpret_cast<const uint4*>(x + j));
+          const uint4 q = __ldcs(reinterpret_cast<const uint4*>(x + j) + 1);
+          const uint32_t u[8] = {w.x, w.y, w.z, w.w, q.x, q.y, q.z, q.w};
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[k][e] = __uint_as_float(u[e]);
         } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] = j + e < V ? static_cast<float>(x[j + e]) : 0.f;
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float v = lp_grad(f[e], z, A, B);
-          if (given && j + e == t) v += gl;
-          f[e] = j + e < V ? v : 0.f;
-        }
-        if constexpr (sizeof(TG) == 4) {
-          float4* o = reinterpret_cast<float4*>(g + j);
-          o[0] = make_float4(f[0], f[1], f[2], f[3]);
-          o[1] = make_float4(f[4], f[5], f[6], f[7]);
-        } else {
-          *reinterpret_cast<uint4*>(g + j) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]),
-                                                        pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+          unpack8_fmt(__ldcs(reinterpret_cast<const uint4*>(x + j)), kFmtBf16, 1.0f, f[k]);
         }
       } else {
-        float f[kPer];
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-          const int j = j0 + e * kLgThreads + threadIdx.x;
-          f[e] = j < V ? static_cast<float>(x[j]) : 0.f;
-        }
+        for (int e = 0; e < 8; ++e) f[k][e] = j + e < V ? static_cast<float>(x[j + e]) : 0.f;
+      }
+    }
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-          const int j = j0 + e * kLgThreads + threadIdx.x;
-          float v = lp_grad(f[e], z, A, B);
-          if (given && j == t) v += gl;
-          if (j >= V) v = 0.f;
-          if (j < cols) {
-            if constexpr (sizeof(TG) == 4) g[j] = v;
-            else g[j] = __float2bfloat16_rn(v);
-          }
-        }
+    for (int k = 0; k < kRounds; ++k) {
+      const int j = j1 + k * kLgThreads * 8;
+      if (j >= cols) break;
+      c.template apply<8>(f[k], j);
+      if (j + 8 > V) {  // padding columns
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (j + e >= V) f[k][e] = 0.f;
+      }
+      if constexpr (sizeof(TG) == 4) {
+        float4* o = reinterpret_cast<float4*>(g + j);
+        o[0] = make_float4(f[k][0], f[k][1], f[k][2], f[k][3]);
+        o[1] = make_float4(f[k][4], f[k][5], f[k][6], f[k][7]);
+      } else {
+        *reinterpret_cast<uint4*>(g + j) = make_uint4(pack_bf16x2(f[k][0], f[k][1]), pack_bf16x2(f[k][2], f[k][3]),
+                                                      pack_bf16x2(f[k][4], f[k][5]), pack_bf16x2(f[k][6], f[k][7]));
       }
     }
   }
 }
 
+template <typename T, typename TG>
+__global__ void __launch_bounds__(kLgThreads)
+    token_logprobs_bwd_any_kernel(const T* __restrict__ logits, int64_t ld, int V,
+                                  const int64_t* __restrict__ targets, const float* __restrict__ lse,
+                                  const float* __restrict__ entropy, const float* __restrict__ g_logp,
+                                  const float* __restrict__ g_entropy, TG* __restrict__ grad,
+                                  int64_t ldg, int cols, int64_t rows) {
+  constexpr int kVE = Row<T>::kVE, kVG = 16 / sizeof(TG);
+  constexpr int kRounds = kLgChunk / kVE / kLgThreads;
+  __shared__ __align__(16) TG buf[kLgChunk];
+  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
+    const Row<T> row(logits + r * ld, V);
+    TG* g = grad + r * ldg;
+    const LpRow c(r, V, targets, lse, entropy, g_logp, g_entropy);
+    // columns [c0, c0 + chunk): c0's gradient is 16-byte aligned (column c0 may
+    // lie before the row)
+    const int c0 = blockIdx.x * kLgChunk - static_cast<int>((reinterpret_cast<uintptr_t>(g) & 15) / sizeof(TG));
+    const int c1 = min(cols, c0 + kLgChunk), stop = min(V, c1);
+    // logit vectors that meet the columns; one more than the chunk holds where both cut it
+    const int i0 = (max(c0, 0) + row.mis) / kVE + threadIdx.x;
+    const int i1 = stop > max(c0, 0) ? (stop + row.mis + kVE - 1) / kVE : 0;
+    float f[kRounds][kVE];
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k)
+      if (i0 + k * kLgThreads < i1) row.load(i0 + k * kLgThreads, f[k]);
+    auto put = [&](float* v, int i) {
+      const int j = row.first(i);
+      c.template apply<kVE>(v, j);
+      if (j >= c0 && j >= 0 && j + kVE <= stop) {
+#pragma unroll
+        for (int e = 0; e < kVE; ++e) buf[j - c0 + e] = to_grad<TG>(v[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kVE; ++e)
+          if (j + e >= max(c0, 0) && j + e < stop) buf[j + e - c0] = to_grad<TG>(v[e]);
+      }
+    };
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k)
+      if (i0 + k * kLgThreads < i1) put(f[k], i0 + k * kLgThreads);
+    for (int i = i0 + kRounds * kLgThreads; i < i1; i += kLgThreads) {
+      row.load(i, f[0]);
+      put(f[0], i);
+    }
+    for (int j = max(V, c0) + threadIdx.x; j < c1; j += kLgThreads) buf[j - c0] = to_grad<TG>(0.f);
+    __syncthreads();
+    for (int v = threadIdx.x; v < kLgChunk / kVG; v += kLgThreads) {
+      const int j = c0 + v * kVG;
+      if (j >= 0 && j + kVG <= c1) {
+        *reinterpret_cast<uint4*>(g + j) = *reinterpret_cast<const uint4*>(buf + v * kVG);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kVG; ++e)
+          if (j + e >= 0 && j + e < c1) g[j + e] = buf[v * kVG + e];
+      }
+    }
+    __syncthreads();
+  }
+}
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-template <typename T, bool kTop>
+template <typename T, bool kTop, int kThreads>
 int launch_fwd(const LogprobsArgs& a, int cluster, cudaStream_t stream) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(a.rows * cluster));
-  cfg.blockDim = dim3(kLpThreads);
+  cfg.blockDim = dim3(kThreads);
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -488,11 +612,25 @@ int launch_fwd(const LogprobsArgs& a, int cluster, cudaStream_t stream) {
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = cluster > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, kTop>, static_cast<const T*>(a.logits),
+  return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, kTop, kThreads>, static_cast<const T*>(a.logits),
                             a.ld, a.V, a.targets, a.top, cluster, a.logp, a.entropy, a.lse,
                             a.top_logp, a.top_ids, a.status) == cudaSuccess
              ? 0
              : 2;
+}
+
+template <typename T>
+int launch_fwd_any(const LogprobsArgs& a, cudaStream_t stream) {
+  // CTAs a row: while the rows leave SMs idle and a CTA's share stays above one
+  // round of its threads' vectors.
+  int cluster = 1;
+  const int64_t vectors = static_cast<int64_t>(a.V) * sizeof(T) / 16;
+  while (cluster < kLpMaxCluster && a.rows * cluster * 2 <= 2 * 148 && vectors / (cluster * 2) >= 512) cluster *= 2;
+  if (a.rows * cluster > 0x7fffffffll) return 1;
+  // 256 threads: 1000 rows of 32768 bf16 logits, 5 alternatives
+  if (a.rows * cluster <= 148)
+    return a.top > 0 ? launch_fwd<T, true, 512>(a, cluster, stream) : launch_fwd<T, false, 512>(a, cluster, stream);
+  return a.top > 0 ? launch_fwd<T, true, 256>(a, cluster, stream) : launch_fwd<T, false, 256>(a, cluster, stream);
 }
 
 template <typename T, typename TG>
@@ -501,16 +639,15 @@ int launch_bwd(const LogprobsBwdArgs& a, cudaStream_t stream) {
   TG* g = static_cast<TG*>(a.grad);
   constexpr int64_t kVT = 16 / sizeof(T), kVG = 16 / sizeof(TG);
   const bool vec = aligned16(x) && aligned16(g) && a.ld % kVT == 0 && a.ldg % kVG == 0 && a.cols % 8 == 0;
-  const int span = kLgThreads * (vec ? 8 : 16);
-  const int64_t bx = (a.cols + span - 1) / span;
-  const int64_t by = std::min<int64_t>(a.rows, 65535);
-  const dim3 grid(static_cast<unsigned>(bx), static_cast<unsigned>(by));
+  const int64_t bx = (a.cols + (vec ? 0 : kVG - 1) + kLgChunk - 1) / kLgChunk;
+  const dim3 grid(static_cast<unsigned>(bx), static_cast<unsigned>(std::min<int64_t>(a.rows, 65535)));
+  const int cols = static_cast<int>(a.cols);
   if (vec)
-    token_logprobs_bwd_kernel<T, TG, true><<<grid, kLgThreads, 0, stream>>>(
-        x, a.ld, a.V, a.targets, a.lse, a.entropy, a.g_logp, a.g_entropy, g, a.ldg, a.cols, a.rows);
+    token_logprobs_bwd_vec_kernel<T, TG><<<grid, kLgThreads, 0, stream>>>(
+        x, a.ld, a.V, a.targets, a.lse, a.entropy, a.g_logp, a.g_entropy, g, a.ldg, cols, a.rows);
   else
-    token_logprobs_bwd_kernel<T, TG, false><<<grid, kLgThreads, 0, stream>>>(
-        x, a.ld, a.V, a.targets, a.lse, a.entropy, a.g_logp, a.g_entropy, g, a.ldg, a.cols, a.rows);
+    token_logprobs_bwd_any_kernel<T, TG><<<grid, kLgThreads, 0, stream>>>(
+        x, a.ld, a.V, a.targets, a.lse, a.entropy, a.g_logp, a.g_entropy, g, a.ldg, cols, a.rows);
   return cudaGetLastError() == cudaSuccess ? 0 : 2;
 }
 
@@ -521,18 +658,7 @@ int token_logprobs(const LogprobsArgs& a, cudaStream_t stream) {
   if (a.rows == 0) return 0;
   const bool bf16 = a.type == kElemBf16;
   if (!bf16 && a.type != kElemF32) return 1;
-  // CTAs a row: while the rows leave SMs idle and a CTA's share stays above one
-  // round of its threads' vectors.
-  int cluster = 1;
-  const int64_t vectors = static_cast<int64_t>(a.V) * (bf16 ? 2 : 4) / 16;
-  while (cluster < kLpMaxCluster && a.rows * cluster * 2 <= 2 * 148 && vectors / (cluster * 2) >= kLpThreads)
-    cluster *= 2;
-  if (a.rows * cluster > 0x7fffffffll) return 1;
-  if (bf16)
-    return a.top > 0 ? launch_fwd<__nv_bfloat16, true>(a, cluster, stream)
-                     : launch_fwd<__nv_bfloat16, false>(a, cluster, stream);
-  return a.top > 0 ? launch_fwd<float, true>(a, cluster, stream)
-                   : launch_fwd<float, false>(a, cluster, stream);
+  return bf16 ? launch_fwd_any<__nv_bfloat16>(a, stream) : launch_fwd_any<float>(a, stream);
 }
 
 int token_logprobs_bwd(const LogprobsBwdArgs& a, cudaStream_t stream) {

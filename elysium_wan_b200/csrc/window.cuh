@@ -2,6 +2,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "pairs.cuh"
 
 namespace ewb {
 
@@ -12,38 +13,6 @@ __device__ __forceinline__ float ex2_wa(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-
-// Pairs of fp32 values in one register pair: one instruction works on both.
-using f32x2 = unsigned long long;
-__device__ __forceinline__ f32x2 pair2(uint32_t lo, uint32_t hi) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
-  return r;
-}
-__device__ __forceinline__ f32x2 pair2(float lo, float hi) {
-  return pair2(__float_as_uint(lo), __float_as_uint(hi));
-}
-__device__ __forceinline__ void unpair2(f32x2 v, float& lo, float& hi) {
-  uint32_t a, b;
-  asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
-  lo = __uint_as_float(a);
-  hi = __uint_as_float(b);
-}
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
 }
 
 // 2^x of a pair on the FMA pipe, for x >= -126 (lower counts as -126): x = n + f
@@ -67,12 +36,6 @@ __device__ __forceinline__ void ex2_poly2(f32x2 x, float& p0, float& p1) {
   unpair2(p, p0, p1);
   p0 = __int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23));
   p1 = __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23));
-}
-
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
 }
 
 // A shared-memory descriptor (sdesc_sw128) moved by `bytes`. One thread issues

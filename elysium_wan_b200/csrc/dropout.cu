@@ -9,11 +9,15 @@
 // 64-bit key is the seed. A mask so depends on (seed, stream, element) alone:
 // not on the launch shape, the strides, the GPU or the pipeline cut.
 //
-// Bound by memory: 2 bytes read for x, 2 for the residual, 2 written (bf16).
-// A block of ten rounds is 20 wide multiplications and 20 three-input xors
-// for four elements, which is under the issue rate left by the copies.
+// Bound by memory with a residual (2 bytes read for x, 2 for the residual, 2
+// written in bf16), by the generator without one: ten rounds are 20 wide
+// multiplications and 20 three-input xors for four elements, of which the first
+// two rounds' halves that do not depend on the block are taken out (philox()),
+// and elements go through the rest in packed pairs. bf16, 16384 x 5120: see the
+// launch for figures.
 #include "common.cuh"
 #include "kernels.h"
+#include "pairs.cuh"
 
 #include <algorithm>
 #include <type_traits>
@@ -22,27 +26,47 @@ namespace ewb {
 namespace {
 
 constexpr int kDropThreads = 256;
+constexpr int kDropPer = 4;  // vectors a thread
 
 struct PhiloxKey {
   uint32_t k0, k1, s0, s1;
 };
 
-__device__ __forceinline__ uint4 philox(uint64_t block, const PhiloxKey& key) {
-  uint32_t c0 = static_cast<uint32_t>(block), c1 = static_cast<uint32_t>(block >> 32);
-  uint32_t c2 = key.s0, c3 = key.s1;
-  uint32_t k0 = key.k0, k1 = key.k1;
+constexpr uint32_t kPhiloxM0 = 0xD2511F53u, kPhiloxM1 = 0xCD9E8D57u;
+constexpr uint32_t kPhiloxW0 = 0x9E3779B9u, kPhiloxW1 = 0xBB67AE85u;
+
+__device__ __forceinline__ uint64_t wide(uint32_t a, uint32_t b) { return static_cast<uint64_t>(a) * b; }
+__device__ __forceinline__ uint32_t hi32(uint64_t v) { return static_cast<uint32_t>(v >> 32); }
+
+// What the blocks of one upper counter word share: of round 1 the product of the
+// stream word, of round 2 the product of what that one and the upper word give.
+struct PhiloxHead {
+  uint64_t b1, a2;
+  __device__ __forceinline__ PhiloxHead(uint32_t upper, const PhiloxKey& key) {
+    b1 = wide(kPhiloxM1, key.s0);
+    a2 = wide(kPhiloxM0, hi32(b1) ^ upper ^ key.k0);
+  }
+};
+
+__device__ __forceinline__ uint4 philox(uint32_t lower, const PhiloxHead& head, const PhiloxKey& key) {
+  const uint64_t a1 = wide(kPhiloxM0, lower);
+  const uint32_t k0 = key.k0 + kPhiloxW0, k1 = key.k1 + kPhiloxW1;
+  const uint64_t b2 = wide(kPhiloxM1, hi32(a1) ^ key.s1 ^ key.k1);
+  uint32_t c0 = hi32(b2) ^ static_cast<uint32_t>(head.b1) ^ k0, c1 = static_cast<uint32_t>(b2);
+  uint32_t c2 = hi32(head.a2) ^ static_cast<uint32_t>(a1) ^ k1, c3 = static_cast<uint32_t>(head.a2);
 #pragma unroll
-  for (int r = 0; r < 10; ++r) {
-    const uint64_t a = static_cast<uint64_t>(0xD2511F53u) * c0;
-    const uint64_t b = static_cast<uint64_t>(0xCD9E8D57u) * c2;
-    c0 = static_cast<uint32_t>(b >> 32) ^ c1 ^ k0;
+  for (int r = 2; r < 10; ++r) {
+    const uint64_t a = wide(kPhiloxM0, c0), b = wide(kPhiloxM1, c2);
+    c0 = hi32(b) ^ c1 ^ (key.k0 + r * kPhiloxW0);
     c1 = static_cast<uint32_t>(b);
-    c2 = static_cast<uint32_t>(a >> 32) ^ c3 ^ k1;
+    c2 = hi32(a) ^ c3 ^ (key.k1 + r * kPhiloxW1);
     c3 = static_cast<uint32_t>(a);
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
   }
   return make_uint4(c0, c1, c2, c3);
+}
+
+__device__ __forceinline__ uint4 philox(uint64_t block, const PhiloxKey& key) {
+  return philox(static_cast<uint32_t>(block), PhiloxHead(hi32(block), key), key);
 }
 
 // ---------------------------------------------------------------- element access
@@ -105,51 +129,68 @@ __device__ __forceinline__ void store8(T* p, const float* v) {
   }
 }
 
-__device__ __forceinline__ float drop(float x, uint32_t word, uint32_t thr, float scale) {
-  return word >= thr ? x * scale : 0.0f;
+// resid + x / (1 - p) of a kept element in one rounding, resid of a dropped one.
+__device__ __forceinline__ float drop_add(float x, uint32_t word, uint32_t thr, float scale, float resid) {
+  return fmaf(word >= thr ? x : 0.f, scale, resid);
 }
 
 // Rows of d elements in vectors of eight (blockIdx.y walks the rows). With
 // more than one row d is a multiple of eight; one row (dense tensors are one
-// row of all their elements) may end in a tail, which the last thread takes.
+// row of all their elements) may end in a tail, which one thread takes. A thread
+// has its kDropPer vectors in flight at once; blocks are short and many, since
+// a grid-wide stride over 1.6 times the resident blocks took 1.2 times as long.
 template <typename TX, typename TR, typename TY, bool kResid>
 __global__ void __launch_bounds__(kDropThreads)
     dropout_vec_kernel(const TX* __restrict__ x, int64_t ldx, const TR* __restrict__ resid,
                        int64_t ldr, TY* __restrict__ y, int64_t ldy, int64_t rows, int64_t d,
                        uint32_t thr, float scale, PhiloxKey key) {
   const int64_t nv = d >> 3;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kDropThreads;
+  const int64_t v0 = static_cast<int64_t>(blockIdx.x) * (kDropThreads * kDropPer) + threadIdx.x;
   for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
     const TX* xr = x + row * ldx;
     const TR* rr = kResid ? resid + row * ldr : nullptr;
     TY* yr = y + row * ldy;
     const uint64_t e0 = static_cast<uint64_t>(row) * d;
-    int64_t v = static_cast<int64_t>(blockIdx.x) * kDropThreads + threadIdx.x;
-    for (; v < nv; v += step) {
-      const Raw8<TX> rx = load8(xr + 8 * v);
-      Raw8<TR> rs;
-      if constexpr (kResid) rs = load8(rr + 8 * v);
-      const uint64_t blk = (e0 >> 2) + 2 * static_cast<uint64_t>(v);
-      const uint4 a = philox(blk, key), b = philox(blk + 1, key);
-      const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-      float f[8], g[8];
-      unpack8(rx, f);
-      if constexpr (kResid) unpack8(rs, g);
+    Raw8<TX> rx[kDropPer];
+    Raw8<TR> rs[kDropPer];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        f[i] = drop(f[i], w[i], thr, scale);
-        if constexpr (kResid) f[i] += g[i];
+    for (int k = 0; k < kDropPer; ++k) {
+      const int64_t v = v0 + k * kDropThreads;
+      if (v < nv) {
+        rx[k] = load8(xr + 8 * v);
+        if constexpr (kResid) rs[k] = load8(rr + 8 * v);
       }
-      store8(yr + 8 * v, f);
     }
-    if (v == nv) {  // the thread after the last whole vector
-      for (int64_t c = 8 * nv; c < d; ++c) {
-        const uint4 a = philox((e0 + c) >> 2, key);
-        const int k = static_cast<int>((e0 + c) & 3);
-        const uint32_t w = k == 0 ? a.x : k == 1 ? a.y : k == 2 ? a.z : a.w;
-        float f = drop(to_f(xr[c]), w, thr, scale);
-        if constexpr (kResid) f += to_f(rr[c]);
-        yr[c] = from_f<TY>(f);
+#pragma unroll
+    for (int k = 0; k < kDropPer; ++k) {
+      const int64_t v = v0 + k * kDropThreads;
+      if (v < nv) {
+        const uint64_t blk = (e0 >> 2) + 2 * static_cast<uint64_t>(v);
+        const PhiloxHead head(hi32(blk), key);  // blk is even: both share the upper word
+        const uint4 a = philox(static_cast<uint32_t>(blk), head, key);
+        const uint4 b = philox(static_cast<uint32_t>(blk) + 1, head, key);
+        const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        float f[8], g[8];
+        unpack8(rx[k], f);
+        if constexpr (kResid) unpack8(rs[k], g);
+        const f32x2 scale2 = pair2(scale, scale);
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          // the choice first, so that what x holds in a dropped place is gone
+          const f32x2 z = pair2(w[i] >= thr ? f[i] : 0.f, w[i + 1] >= thr ? f[i + 1] : 0.f);
+          if constexpr (kResid) unpair2(fma2(z, scale2, pair2(g[i], g[i + 1])), f[i], f[i + 1]);
+          else unpair2(mul2(z, scale2), f[i], f[i + 1]);
+        }
+        store8(yr + 8 * v, f);
+      } else if (v == nv) {  // the place after the last whole vector
+        for (int64_t c = 8 * nv; c < d; ++c) {
+          const uint4 a = philox((e0 + c) >> 2, key);
+          const int z = static_cast<int>((e0 + c) & 3);
+          const uint32_t w = z == 0 ? a.x : z == 1 ? a.y : z == 2 ? a.z : a.w;
+          float g = 0.f;
+          if constexpr (kResid) g = to_f(rr[c]);
+          yr[c] = from_f<TY>(drop_add(to_f(xr[c]), w, thr, scale, g));
+        }
       }
     }
   }
@@ -171,9 +212,9 @@ __global__ void __launch_bounds__(kDropThreads)
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       if (4 * b + k >= n) break;
-      float f = drop(to_f(x[row * ldx + col]), w[k], thr, scale);
-      if constexpr (kResid) f += to_f(resid[row * ldr + col]);
-      y[row * ldy + col] = from_f<TY>(f);
+      float g = 0.f;
+      if constexpr (kResid) g = to_f(resid[row * ldr + col]);
+      y[row * ldy + col] = from_f<TY>(drop_add(to_f(x[row * ldx + col]), w[k], thr, scale, g));
       if (++col == d) {
         col = 0;
         ++row;
@@ -200,15 +241,15 @@ int launch(const DropoutArgs& a, cudaStream_t stream) {
   // 16-byte vectors need aligned bases and, from row to row, aligned steps
   const bool bases = aligned16(x) && aligned16(y) && (!kResid || aligned16(r));
   const bool steps = rows == 1 || (d % 8 == 0 && ldx % 8 == 0 && ldy % 8 == 0 && (!kResid || ldr % 8 == 0));
-  const int64_t most = 148 * 8;  // every resident block of an SM
   if (bases && steps) {
-    const int64_t bx = std::max<int64_t>(1, std::min<int64_t>((d / 8 + kDropThreads) / kDropThreads, most));
-    const int64_t by = std::min<int64_t>(rows, std::max<int64_t>(1, 4 * most / bx));
+    const int64_t bx = d / 8 / (kDropThreads * kDropPer) + 1;  // one place more than whole vectors
+    if (bx > 0x7fffffff) return 1;
+    const int64_t by = std::min<int64_t>(rows, 65535);
     dropout_vec_kernel<TX, TR, TY, kResid>
         <<<dim3(static_cast<unsigned>(bx), static_cast<unsigned>(by)), kDropThreads, 0, stream>>>(
             x, ldx, r, ldr, y, ldy, rows, d, a.thr, a.scale, key);
   } else {
-    const int64_t bx = std::min<int64_t>((rows * d / 4 + kDropThreads) / kDropThreads, 4 * most);
+    const int64_t bx = std::min<int64_t>((rows * d / 4 + kDropThreads) / kDropThreads, 148 * 64);
     dropout_any_kernel<TX, TR, TY, kResid><<<static_cast<unsigned>(bx), kDropThreads, 0, stream>>>(
         x, ldx, r, ldr, y, ldy, rows, d, a.thr, a.scale, key);
   }

@@ -9,16 +9,20 @@
 // A cache that never fills is the same rule without a wrap.
 //
 // Bound by memory: every visible row is read once (4 Hkv hd bytes). One cluster
-// of 1 to 8 CTAs serves one (sequence, kv head, up to 16 of its query heads);
-// its warps take groups of 16 visible rows in turn, straight from global memory
-// into mma fragments, with a softmax of their own each (running maximum and sum in
-// fp32); warps join in shared memory, CTAs through distributed shared memory,
-// both in a fixed order. The contraction order of q.k is free, so a lane's 16
-// bytes of a key row serve two k-steps of m16n8k16 as they lie, and a value
-// row's 16 bytes serve eight column tiles; neither needs a transpose. The
-// legacy mma is enough here: at 16 query rows it runs at a few per cent.
-// p is split into two bf16 terms (p = hi + lo), so the second product keeps
-// about 16 bits of each weight; the tensor pipe idles anyway.
+// of 1 to 8 CTAs serves one (sequence, kv head, up to 8 of its query heads); its
+// warps take groups of 16 visible rows in turn, straight from global memory into
+// mma fragments, with a softmax of their own each (running maximum and sum in fp32);
+// warps join in shared memory, CTAs through distributed shared memory, both in a
+// fixed order. Only other warps cover a warp's loads (4 to 8 KB a group), so CTAs
+// are of four warps and several share an SM.
+//
+// Both products have the 16 rows (or 16 columns of the head) as the m of m16n8k16 and
+// the query heads as its n: S^T = K Q^T and O^T = V^T P^T. The contraction order
+// of q.k is free, so a lane's 16 bytes of a key row serve two k-steps as they lie; a
+// lane's 16 bytes of four value rows serve four column tiles after one byte
+// permutation each; P^T turns from result to operand by movmatrix. The legacy
+// mma is enough here: it runs at a few per cent. p is split into two bf16 terms
+// (p = hi + lo), so the second product keeps about 16 bits of each weight.
 #include "common.cuh"
 #include "kernels.h"
 
@@ -27,9 +31,9 @@
 namespace ewb {
 namespace {
 
-constexpr int kStWarps = 8;
+constexpr int kStWarps = 4;
 constexpr int kStThreads = kStWarps * 32;
-constexpr int kStHeads = 16;  // query heads of one CTA (the m of the mma)
+constexpr int kStHeads = 8;   // query heads of one CTA (the n of the mma)
 constexpr int kStKeys = 16;   // rows of one group
 constexpr float kLog2eSt = 1.4426950408889634f;
 
@@ -122,15 +126,25 @@ struct ValFrag {
     }
     if constexpr (kRest == 2) w[4 * kFull] = ld4_st(row + 64 * kFull + 2 * g);
   }
-  // The column of the row that tile t, mma column n holds.
-  __device__ static __forceinline__ int column(int t, int n) {
-    return t < 8 * kFull ? 64 * (t / 8) + 8 * n + t % 8
-                         : 64 * kFull + kRest * n + (t - 8 * kFull);
+  // The column of the head that row n (0-7) of half z of 16-column tile t is:
+  // the two halves are the low and high half of word t.
+  __device__ static __forceinline__ int column(int t, int z, int n) {
+    return t < 4 * kFull ? 64 * (t / 4) + 8 * n + 2 * (t % 4) + z : 64 * kFull + kRest * n + 2 * (t - 4 * kFull) + z;
   }
 };
 
+// An 8 x 8 matrix of 16-bit values, one row of pairs a lane quad, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// CTAs an SM that the registers allow for.
+__host__ __device__ constexpr int step_ctas(int hd) { return hd <= 64 ? 5 : hd <= 96 ? 4 : 3; }
+
 template <int HD>
-__global__ void __launch_bounds__(kStThreads, 1)
+__global__ void __launch_bounds__(kStThreads, step_ctas(HD))
     window_step_kernel(const __nv_bfloat16* __restrict__ qkv, int64_t ldq, __nv_bfloat16* cache,
                        int64_t stride_b, int64_t stride_s, const int64_t* __restrict__ pos,
                        __nv_bfloat16* __restrict__ o, int H, int Hkv, int htiles, int cluster,
@@ -138,7 +152,7 @@ __global__ void __launch_bounds__(kStThreads, 1)
   extern __shared__ float st_smem[];  // [warps][rows][HD] partial outputs
   __shared__ float sh_m[kStWarps][kStHeads], sh_l[kStWarps][kStHeads];
   __shared__ float cta_m[kStHeads], cta_l[kStHeads];
-  constexpr int kTiles = HD / 8;
+  constexpr int kTiles = HD / 16;
 
   const int part = blockIdx.x % cluster;
   int64_t rest = blockIdx.x / cluster;
@@ -178,19 +192,16 @@ __global__ void __launch_bounds__(kStThreads, 1)
     return base + s * stride_s;
   };
 
-  KeyFrag<HD> qa, qb;  // query heads g and g + 8
-  qa.zero();
-  qb.zero();
-  const __nv_bfloat16* qrow = qkv + b * ldq + static_cast<int64_t>(h0) * HD;
-  if (g < rows) qa.load(qrow + g * HD, q);
-  if (g + 8 < rows) qb.load(qrow + (g + 8) * HD, q);
+  KeyFrag<HD> qf;  // query head g
+  qf.zero();
+  if (g < rows) qf.load(qkv + b * ldq + static_cast<int64_t>(h0 + g) * HD, q);
 
   float acc[kTiles][4];
 #pragma unroll
   for (int t = 0; t < kTiles; ++t)
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
-  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // of heads 2q, 2q + 1
 
   const int groups = (n + kStKeys - 1) / kStKeys, all_warps = cluster * kStWarps;
   for (int G = part * kStWarps + warp; G < groups; G += all_warps) {
@@ -202,91 +213,65 @@ __global__ void __launch_bounds__(kStThreads, 1)
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       v[e].load(row(min(i0 + 2 * q + (e & 1) + 8 * (e >> 1), n - 1)) + kv_off, g);
-    float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+    float s[4] = {0.f, 0.f, 0.f, 0.f};  // rows g, g + 8 x heads 2q, 2q + 1
 #pragma unroll
     for (int c = 0; c < KeyFrag<HD>::kFull; ++c) {
-      mma_st(s0, qa.w[c].x, qb.w[c].x, qa.w[c].y, qb.w[c].y, k0.w[c].x, k0.w[c].y);
-      mma_st(s1, qa.w[c].x, qb.w[c].x, qa.w[c].y, qb.w[c].y, k1.w[c].x, k1.w[c].y);
-      mma_st(s0, qa.w[c].z, qb.w[c].z, qa.w[c].w, qb.w[c].w, k0.w[c].z, k0.w[c].w);
-      mma_st(s1, qa.w[c].z, qb.w[c].z, qa.w[c].w, qb.w[c].w, k1.w[c].z, k1.w[c].w);
+      mma_st(s, k0.w[c].x, k1.w[c].x, k0.w[c].y, k1.w[c].y, qf.w[c].x, qf.w[c].y);
+      mma_st(s, k0.w[c].z, k1.w[c].z, k0.w[c].w, k1.w[c].w, qf.w[c].z, qf.w[c].w);
     }
-    if constexpr (KeyFrag<HD>::kHalf) {
-      mma_st(s0, qa.t.x, qb.t.x, qa.t.y, qb.t.y, k0.t.x, k0.t.y);
-      mma_st(s1, qa.t.x, qb.t.x, qa.t.y, qb.t.y, k1.t.x, k1.t.y);
-    }
-    // this lane: rows g (x0) and g + 8 (x1), keys 2q, 2q + 1, 2q + 8, 2q + 9
-    float x0[4] = {s0[0], s0[1], s1[0], s1[1]}, x1[4] = {s0[2], s0[3], s1[2], s1[3]};
-    float mx0 = -INFINITY, mx1 = -INFINITY;
+    if constexpr (KeyFrag<HD>::kHalf) mma_st(s, k0.t.x, k1.t.x, k0.t.y, k1.t.y, qf.t.x, qf.t.y);
+    const bool in0 = i0 + g < n, in1 = i0 + 8 + g < n;
+    float a[2];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const bool ok = i0 + 2 * q + (e & 1) + 8 * (e >> 1) < n;
-      x0[e] = ok ? x0[e] * scale_log2 : -INFINITY;
-      x1[e] = ok ? x1[e] * scale_log2 : -INFINITY;
-      mx0 = fmaxf(mx0, x0[e]);
-      mx1 = fmaxf(mx1, x1[e]);
-    }
+    for (int z = 0; z < 2; ++z) {
+      s[z] = in0 ? s[z] * scale_log2 : -INFINITY;
+      s[2 + z] = in1 ? s[2 + z] * scale_log2 : -INFINITY;
+      float mx = fmaxf(s[z], s[2 + z]);
 #pragma unroll
-    for (int d = 1; d < 4; d <<= 1) {
-      mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, d));
-      mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, d));
+      for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+      // a group has a visible row, so the maximum is finite (or the data is not)
+      const float mn = fmaxf(m[z], mx);
+      a[z] = m[z] == -INFINITY ? 0.f : ex2_st(m[z] - mn);
+      m[z] = mn;
+      s[z] = ex2_st(s[z] - mn);
+      s[2 + z] = ex2_st(s[2 + z] - mn);
+      l[z] = l[z] * a[z] + (s[z] + s[2 + z]);
     }
-    // a group has a visible row, so the maxima are finite (or the data is not)
-    const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
-    const float a0 = m0 == -INFINITY ? 0.f : ex2_st(m0 - n0);
-    const float a1 = m1 == -INFINITY ? 0.f : ex2_st(m1 - n1);
-    m0 = n0;
-    m1 = n1;
-    float r0 = 0.f, r1 = 0.f;
+    uint32_t ph[2], pl[2];
+    split2(s[0], s[1], ph[0], pl[0]);
+    split2(s[2], s[3], ph[1], pl[1]);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      x0[e] = ex2_st(x0[e] - n0);
-      x1[e] = ex2_st(x1[e] - n1);
-      r0 += x0[e];
-      r1 += x1[e];
+    for (int z = 0; z < 2; ++z) {
+      ph[z] = transpose8(ph[z]);
+      pl[z] = transpose8(pl[z]);
     }
-    l0 = l0 * a0 + r0;
-    l1 = l1 * a1 + r1;
-    uint32_t ph[4], pl[4];
-    split2(x0[0], x0[1], ph[0], pl[0]);
-    split2(x1[0], x1[1], ph[1], pl[1]);
-    split2(x0[2], x0[3], ph[2], pl[2]);
-    split2(x1[2], x1[3], ph[3], pl[3]);
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) {
-      acc[t][0] *= a0;
-      acc[t][1] *= a0;
-      acc[t][2] *= a1;
-      acc[t][3] *= a1;
-      const int wi = t / 2;
-      const uint32_t sel = (t & 1) ? 0x7632u : 0x5410u;
-      const uint32_t b0 = __byte_perm(v[0].w[wi], v[1].w[wi], sel);
-      const uint32_t b1 = __byte_perm(v[2].w[wi], v[3].w[wi], sel);
-      mma_st(acc[t], ph[0], ph[1], ph[2], ph[3], b0, b1);
-      mma_st(acc[t], pl[0], pl[1], pl[2], pl[3], b0, b1);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[t][e] *= a[e & 1];
+      const uint32_t a0 = __byte_perm(v[0].w[t], v[1].w[t], 0x5410u), a1 = __byte_perm(v[0].w[t], v[1].w[t], 0x7632u);
+      const uint32_t a2 = __byte_perm(v[2].w[t], v[3].w[t], 0x5410u), a3 = __byte_perm(v[2].w[t], v[3].w[t], 0x7632u);
+      mma_st(acc[t], a0, a1, a2, a3, ph[0], ph[1]);
+      mma_st(acc[t], a0, a1, a2, a3, pl[0], pl[1]);
     }
   }
 
   // ---- join the warps of this CTA
 #pragma unroll
-  for (int d = 1; d < 4; d <<= 1) {
-    l0 += __shfl_xor_sync(0xffffffffu, l0, d);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, d);
-  }
-  if (q == 0) {
-    sh_m[warp][g] = m0;
-    sh_m[warp][g + 8] = m1;
-    sh_l[warp][g] = l0;
-    sh_l[warp][g + 8] = l1;
+  for (int z = 0; z < 2; ++z) {
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1) l[z] += __shfl_xor_sync(0xffffffffu, l[z], d);
+    if (g == 0) {
+      sh_m[warp][2 * q + z] = m[z];
+      sh_l[warp][2 * q + z] = l[z];
+    }
   }
   float* mine = st_smem + warp * rows * HD;
 #pragma unroll
   for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int col = ValFrag<HD>::column(t, 2 * q + e);
-      if (g < rows) mine[g * HD + col] = acc[t][e];
-      if (g + 8 < rows) mine[(g + 8) * HD + col] = acc[t][2 + e];
-    }
+    for (int e = 0; e < 4; ++e)
+      if (2 * q + (e & 1) < rows) mine[(2 * q + (e & 1)) * HD + ValFrag<HD>::column(t, e >> 1, g)] = acc[t][e];
   __syncthreads();
   for (int i = threadIdx.x; i < rows * HD; i += kStThreads) {
     const int r = i / HD;
@@ -345,19 +330,17 @@ int launch_step(const WindowStepArgs& a, cudaStream_t stream) {
   const int rep = a.H / a.Hkv, htiles = (rep + kStHeads - 1) / kStHeads;
   const int64_t units = a.B * a.Hkv * htiles;
   const int64_t visible = std::min<int64_t>(a.cap, static_cast<int64_t>(std::min(a.window, a.cap - a.sinks)) + a.sinks);
-  // CTAs a unit: while the units leave SMs idle and every warp keeps a group
+  // CTAs a unit: up to about two rounds of what the SMs hold at once, so that the
+  // last one is not a large part of all, while every warp keeps two groups of rows.
+  // 8 x 40 heads x 128 over 4160 rows: 127 us at one round, 85 at two, 84 at four;
+  // 48 x 8 heads x 64 over 2063 rows: 52, 36, 40.
   int cluster = 1;
-  while (cluster < 8 && units * cluster * 2 <= 2 * 148 && visible >= static_cast<int64_t>(cluster) * 2 * kStWarps * kStKeys)
+  const int64_t room = 2 * 148 * step_ctas(HD);
+  while (cluster < 8 && units * cluster * 2 <= room &&
+         visible >= static_cast<int64_t>(cluster) * 2 * kStWarps * kStKeys * 2)
     cluster *= 2;
   if (units * cluster > 0x7fffffffll) return 1;
   const size_t smem = static_cast<size_t>(kStWarps) * std::min(rep, kStHeads) * HD * sizeof(float);
-  static bool attr = false;
-  if (!attr) {
-    if (cudaFuncSetAttribute(window_step_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             kStWarps * kStHeads * HD * static_cast<int>(sizeof(float))) != cudaSuccess)
-      return 2;
-    attr = true;
-  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(units * cluster));
   cfg.blockDim = dim3(kStThreads);

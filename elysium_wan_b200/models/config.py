@@ -55,6 +55,14 @@ class GPTConfig:
     n_kv_head: int | None = None
     rope_theta: float = 10000.0
     rms_eps: float = 1e-6
+    # Long texts (this engine's own fields): a query sees the last attn_window
+    # positions and the first attn_sinks ones; None = full causal attention.
+    attn_window: int | None = None
+    attn_sinks: int = 0
+    # Residual dropout: each block adds x * keep / (1 - dropout) of its two
+    # branches to the stream. The mask is a function of (seed, step, microbatch,
+    # entry, branch, element), so no cut, width or recompute changes it.
+    dropout: float = 0.0
     lora_rank: int = 0
     lora_alpha: float = 16.0
     lora_targets: str = "attn"  # attn | attn_mlp | all
@@ -148,6 +156,8 @@ class GPTConfig:
                 raise ValueError("user models run in fp32 with fp32 boundaries (the host path)")
             if self.lora_rank or self.moe_experts or self.tie_embeddings:
                 raise ValueError("LoRA, MoE and tied embeddings are built-in decoder knobs")
+            if self.attn_window is not None or self.dropout:
+                raise ValueError("attn_window and dropout are built-in decoder knobs")
         elif self.arch != "builtin":
             raise NotImplementedError(
                 f"arch {self.arch!r}: this engine builds the built-in decoder family and user "
@@ -163,6 +173,12 @@ class GPTConfig:
             raise ValueError("rope needs an even head_dim")
         if self.tie_embeddings and self.init_scheme != "gpt2":
             raise ValueError("tie_embeddings requires init_scheme='gpt2' (one scale for both uses)")
+        if self.attn_window is not None and self.attn_window < 1:
+            raise ValueError(f"attn_window={self.attn_window} must be at least 1 (None = full)")
+        if self.attn_sinks < 0 or (self.attn_sinks and self.attn_window is None):
+            raise ValueError("attn_sinks must be at least 0, and needs attn_window")
+        if not 0.0 <= self.dropout < 1.0:
+            raise ValueError(f"dropout={self.dropout} is not in [0, 1)")
         if self.lora_rank < 0:
             raise ValueError("lora_rank must be >= 0")
         if self.fp8_boundary() and self.d_model % 128:

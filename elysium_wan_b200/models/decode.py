@@ -1,0 +1,145 @@
+"""Scoring and answering with a trained model, on one device.
+
+``Decoder`` reads a whole StageModel (every entry on one device) without dropout:
+
+  * ``score``: the log probability of every given token of a text, the entropy of
+    every prediction and its most probable alternatives;
+  * ``prefill`` / ``step``: an answer token by token. A model with ``attn_window``
+    keeps its keys and values in rings of attn_sinks + attn_window rows a layer
+    and sequence, so an answer may be of any length (learned positions end at
+    seq_len; rotary ones do not); a full-attention model keeps seq_len rows.
+
+Logits are made and read in blocks of rows, so the fp32 logits of a long text are
+never held whole.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from elysium_wan_b200 import ops
+
+from .gpt import Block, StageModel, _boundary_out
+
+
+class Decoder:
+    def __init__(self, model: StageModel, logit_rows: int = 2048):
+        c = model.cfg
+        if not (model.first and model.last) or c.arch == "user" or c.moe_experts:
+            raise ValueError("Decoder needs every entry of a dense built-in model on one device")
+        self.model, self.cfg, self.rows = model, c, logit_rows
+        self.cuda = model.device.type == "cuda"
+        self.embed, *self.blocks, self.head = model.layers
+        self.window = c.attn_window or c.seq_len
+        self.slots = c.attn_sinks + self.window
+
+    # ------------------------------------------------------------- whole texts
+    def _logits_of(self, y):
+        w, V = self.model.store.w(self.head.out), self.cfg.vocab_size
+        if not self.cuda:
+            return ops.linear_fwd(y, w, epi="f32")
+        # rows of a multiple of four columns, as the GEMM stores them
+        out = torch.empty((y.shape[0], (V + 7) // 8 * 8), dtype=torch.float32, device=y.device)
+        ops.linear_fwd(y, w, epi="f32", out=out[:, :V])
+        return out
+
+    def _final_norm(self, x, scale):
+        c, s, h = self.cfg, self.model.store, self.head
+        beta = None if h.rms else s.p(h.n("ln_f.bias"))
+        return ops.layernorm_fwd(x, scale, s.p(h.n("ln_f.weight")), beta, c.norm_eps)[0]
+
+    def hidden(self, tokens):
+        """The final activations of tokens [B, seq_len]."""
+        if tokens.dim() != 2 or tokens.shape[1] != self.cfg.seq_len:
+            raise ValueError(f"texts come as [B, {self.cfg.seq_len}] tokens (pad shorter ones)")
+        x = self.embed.forward(tokens.contiguous(), {})
+        for b in self.blocks:
+            x = b.forward(x, {})
+        return x
+
+    def score(self, tokens, targets, *, top: int = 0) -> ops.TokenLogprobs:
+        """Statistics of the predictions made at tokens [B, seq_len]: log
+        probabilities of targets [B, seq_len] (negative: none given), entropy and
+        `top` alternatives, all [B * seq_len, ...]."""
+        c = self.cfg
+        x = self.hidden(tokens)
+        y = self._final_norm(x.x, x.scale)
+        t = targets.reshape(-1)
+        parts = [ops.token_logprobs(self._logits_of(y[a:a + self.rows]), c.vocab_size,
+                                    t[a:a + self.rows].contiguous(), top=top)
+                 for a in range(0, y.shape[0], self.rows)]
+        return ops.TokenLogprobs(*(torch.cat(v) if v[0] is not None else None for v in zip(*parts)))
+
+    # ------------------------------------------------------------- answers
+    def new_caches(self, B: int) -> list:
+        """One ring a layer: [B, sinks + window, 2 * kv_heads * head_dim]."""
+        c = self.cfg
+        dt = torch.bfloat16 if self.cuda else torch.float32
+        return [torch.zeros((B, self.slots, 2 * c.kv_heads * c.head_dim), dtype=dt,
+                            device=self.model.device) for _ in self.blocks]
+
+    def prefill(self, tokens, lengths, caches):
+        """Put prompts [B, seq_len] of the given lengths (int32 [B]) into the
+        rings. Returns the positions [B] of the next tokens (the lengths)."""
+        c = self.cfg
+        B, S = tokens.shape
+        x = self.embed.forward(tokens.contiguous(), {})
+        for b, cache in zip(self.blocks, caches):
+            ctx: dict = {}
+            x = b.forward(x, ctx)
+            ops.window_cache_fill(ctx["qkv"], cache, B, S, c.n_head, c.head_dim, c.kv_heads,
+                                  sinks=c.attn_sinks, lengths=lengths)
+        return lengths.to(torch.int64)
+
+    def _angles(self, pos):
+        """(cos, sin) [B, head_dim / 2] at the rows' positions, formed in fp64 as
+        the tables are."""
+        c = self.cfg
+        inv = c.rope_theta ** (-torch.arange(0, c.head_dim, 2, dtype=torch.float64, device=pos.device)
+                               / c.head_dim)
+        a = pos.clamp(min=0).double()[:, None] * inv
+        return torch.cos(a).float(), torch.sin(a).float()
+
+    def _boundary(self, y):
+        """An entry's output as the next one reads it in training: rounded to the
+        boundary format."""
+        q8 = ops.q8_dtype(self.cfg.boundary_dtype)
+        if q8 is not None:
+            return ops.dequant_q8(*ops.quant_q8(y, q8), torch.bfloat16 if self.cuda else torch.float32)
+        if self.cuda:
+            return y.to(ops.act_dtype(self.cfg.boundary_dtype, True))
+        return _boundary_out(self.cfg, y).x
+
+    def step(self, tokens, pos, caches, *, top: int = 1) -> ops.TokenLogprobs:
+        """One token a sequence: tokens [B] at positions pos [B] (negative: idle)
+        enter the rings; returns the statistics of the next token's prediction
+        (top_ids[:, 0] is the most probable one)."""
+        c, s = self.cfg, self.model.store
+        if (c.pos == "learned" or c.attn_window is None) and int(pos.max()) >= c.seq_len:
+            raise ValueError(f"learned positions and full attention end at seq_len={c.seq_len}; "
+                             f"longer answers need attn_window and rotary positions")
+        x = ops.embed_fwd(tokens, s.p("0.tok.weight"), None, 1,
+                          out_dtype=torch.bfloat16 if self.cuda else torch.float32)
+        if c.pos == "learned":
+            x = (x.float() + s.p("0.pos.weight")[pos.clamp(min=0)]).to(x.dtype)
+        x = self._boundary(x)
+        turn = self._angles(pos) if c.pos == "rope" else None
+        for b, cache in zip(self.blocks, caches):
+            x = self._block_step(b, x, pos, turn, cache)
+        return ops.token_logprobs(self._logits_of(self._final_norm(x, None)), c.vocab_size, top=top)
+
+    def _block_step(self, b: Block, x, pos, turn, cache):
+        c, s = self.cfg, self.model.store
+        h1, _, _ = b._norm(x, None, "ln1")
+        qkv = ops.linear_fwd(h1, b._w(b.qkv_w), b._bp(b.qkv_b))
+        if turn is not None:
+            ops.rope_rows(qkv, c.d_model + c.kv_heads * c.head_dim, c.head_dim, *turn)
+        o = ops.window_attention_step(qkv, cache, pos, c.n_head, c.head_dim, c.kv_heads,
+                                      window=self.window, sinks=c.attn_sinks)
+        x2 = ops.linear_fwd(o, s.w(b.n("proj.weight")), b._bp([b.n("proj.bias")]), epi="resid", resid=x)
+        h2, _, _ = b._norm(x2, None, "ln2")
+        if b.mlp == "gelu":
+            hin, _ = ops.linear_fwd(h2, b._w(b.up_w), b._bp(b.up_b), epi="gelu")
+        else:
+            hin = ops.swiglu_fwd(ops.linear_fwd(h2, b._w(b.up_w), b._bp(b.up_b)))
+        return self._boundary(ops.linear_fwd(hin, s.w(b.dn_w), b._bp([b.dn_b]), epi="resid", resid=x2))

@@ -384,8 +384,9 @@ class Block:
     rotary positions on q and k, GELU or SwiGLU MLP or the MoE block, biases
     optional."""
 
-    def __init__(self, cfg, store: ParamStore, e: int):
+    def __init__(self, cfg, store: ParamStore, e: int, seed: int = 0):
         self.cfg, self.s, self.e = cfg, store, e
+        self.seed = seed & ((1 << 64) - 1)  # of the dropout masks
         self.n = lambda k: f"{e}.{k}"
         n = self.n
         gen = uses_general_arch(cfg)
@@ -453,24 +454,56 @@ class Block:
         return ops.layernorm_bwd(dy, x, xs, m, r, s.p(n(f"{which}.weight")), dres, dg, dbeta,
                                  accumulate=True)
 
+    def attention(self, qkv, B, S):
+        """(o, lse) over packed rows, in the configured window."""
+        c = self.cfg
+        if c.attn_window is None:
+            return ops.attention_fwd(qkv, B, S, c.n_head, c.head_dim, c.kv_heads)
+        return ops.window_attention_fwd(qkv, B, S, c.n_head, c.head_dim, c.kv_heads,
+                                        window=c.attn_window, sinks=c.attn_sinks)
+
+    def _stream(self, draw: int, branch: int) -> int:
+        """The dropout stream of one microbatch (draw numbers it in the run)."""
+        return (draw * self.cfg.n_entries + self.e) * 2 + branch
+
+    def _drop_add(self, y, resid: Act, draw, branch, out_dtype):
+        r = resid.x
+        if resid.fp8:
+            r = ops.dequant_q8(r, resid.scale, torch.bfloat16 if r.is_cuda else torch.float32)
+        return ops.dropout_add(y, r, self.cfg.dropout, self.seed, self._stream(draw, branch),
+                               out_dtype=out_dtype)
+
+    def _drop_bwd(self, dy, ctx, branch):
+        if ctx.get("draw") is None:
+            return dy
+        return ops.dropout_bwd(dy, self.cfg.dropout, self.seed, self._stream(ctx["draw"], branch))
+
     def forward(self, x: Act, ctx: dict) -> Act:
         c, s, n = self.cfg, self.s, self.n
         T = x.rows
-        B, S, H, hd = T // c.seq_len, c.seq_len, c.n_head, c.head_dim
+        B, S, hd = T // c.seq_len, c.seq_len, c.head_dim
+        draw = ctx.get("draw")  # None: no dropout
         h1, m1, r1 = self._norm(x.x, x.scale, "ln1")
         qkv = ops.linear_fwd(h1, self._w(self.qkv_w), self._bp(self.qkv_b))
         if c.pos == "rope":
             ops.rope(qkv, S, c.d_model + c.kv_heads * hd, hd, c.rope_theta)
-        o, lse = ops.attention_fwd(qkv, B, S, H, hd, c.kv_heads)
-        x2 = ops.linear_fwd(o, s.w(n("proj.weight")), self._bp([n("proj.bias")]), epi="resid",
-                            resid=x.x, resid_scale=x.scale)
+        o, lse = self.attention(qkv, B, S)
+        if draw is None:
+            x2 = ops.linear_fwd(o, s.w(n("proj.weight")), self._bp([n("proj.bias")]), epi="resid",
+                                resid=x.x, resid_scale=x.scale)
+        else:
+            y = ops.linear_fwd(o, s.w(n("proj.weight")), self._bp([n("proj.bias")]))
+            x2 = self._drop_add(y, x, draw, 0, ops.act_dtype("bf16", y.is_cuda))
         h2, m2, r2 = self._norm(x2, None, "ln2")
         ctx.update(x=x, h1=h1, m1=m1, r1=r1, qkv=qkv, o=o, lse=lse, x2=x2, h2=h2, m2=m2, r2=r2)
         q8 = ops.q8_dtype(c.boundary_dtype)
         out_dt = ops.act_dtype(c.boundary_dtype, x2.is_cuda)
         if self.mlp == "moe":
             y = self.moe.forward(h2, ctx)
-            out = ops.residual_add(x2, y)  # x2 + y in the compute dtype
+            if draw is not None:
+                out = self._drop_add(y, Act(x2), draw, 1, x2.dtype)
+            else:
+                out = ops.residual_add(x2, y)  # x2 + y in the compute dtype
             if q8 is not None:
                 return Act(*ops.quant_q8(out, q8))
             if out.is_cuda and out.dtype != out_dt:
@@ -485,6 +518,11 @@ class Block:
             hin = ops.swiglu_fwd(gu)
             ctx.update(gu=gu, g=hin)
         bdn = self._bp([self.dn_b])
+        if draw is not None:
+            y = ops.linear_fwd(hin, s.w(self.dn_w), bdn)
+            if q8 is not None:
+                return Act(*ops.quant_q8(self._drop_add(y, Act(x2), draw, 1, x2.dtype), q8))
+            return _boundary_out(c, self._drop_add(y, Act(x2), draw, 1, out_dt))
         if q8 is not None:
             q, sc = ops.linear_fwd(hin, s.w(self.dn_w), bdn, epi="resid_q8", resid=x2, q8=q8)
             return Act(q, sc)
@@ -496,25 +534,31 @@ class Block:
         T = dy.shape[0]
         B, S, H, hd = T // c.seq_len, c.seq_len, c.n_head, c.head_dim
         x: Act = ctx["x"]
+        db = self._drop_bwd(dy, ctx, 1)  # the gradient of the MLP branch
         if self.mlp == "moe":
-            dh2 = self.moe.backward(ctx, dy, wq)
+            dh2 = self.moe.backward(ctx, db, wq)
         elif self.mlp == "gelu":
-            du = ops.linear_dx(dy, s.w(self.dn_w), gelu_u=ctx["u"])
-            wq += w_tasks(s, dy, ctx["g"], [self.dn_w], self._bn([self.dn_b]), self.lora_s)
+            du = ops.linear_dx(db, s.w(self.dn_w), gelu_u=ctx["u"])
+            wq += w_tasks(s, db, ctx["g"], [self.dn_w], self._bn([self.dn_b]), self.lora_s)
             dh2 = ops.linear_dx(du, self._w(self.up_w))
             wq += w_tasks(s, du, ctx["h2"], self.up_w, self._bn(self.up_b), self.lora_s)
         else:
-            dh = ops.linear_dx(dy, s.w(self.dn_w))
-            wq += w_tasks(s, dy, ctx["g"], [self.dn_w], self._bn([self.dn_b]), self.lora_s)
+            dh = ops.linear_dx(db, s.w(self.dn_w))
+            wq += w_tasks(s, db, ctx["g"], [self.dn_w], self._bn([self.dn_b]), self.lora_s)
             dgu = ops.swiglu_bwd(dh, ctx["gu"])
             del dh
             dh2 = ops.linear_dx(dgu, self._w(self.up_w))
             wq += w_tasks(s, dgu, ctx["h2"], self.up_w, self._bn(self.up_b), self.lora_s)
         dx2 = self._norm_bwd(dh2, ctx["x2"], None, ctx["m2"], ctx["r2"], "ln2", dy)
-        do = ops.linear_dx(dx2, s.w(n("proj.weight")))
-        wq += w_tasks(s, dx2, ctx["o"], [n("proj.weight")], self._bn([n("proj.bias")]),
+        db = self._drop_bwd(dx2, ctx, 0)  # the gradient of the attention branch
+        do = ops.linear_dx(db, s.w(n("proj.weight")))
+        wq += w_tasks(s, db, ctx["o"], [n("proj.weight")], self._bn([n("proj.bias")]),
                       self.lora_s)
-        dqkv = ops.attention_bwd(ctx["qkv"], ctx["o"], do, ctx["lse"], B, S, H, hd, c.kv_heads)
+        if c.attn_window is None:
+            dqkv = ops.attention_bwd(ctx["qkv"], ctx["o"], do, ctx["lse"], B, S, H, hd, c.kv_heads)
+        else:
+            dqkv = ops.window_attention_bwd(ctx["qkv"], ctx["o"], do, ctx["lse"], B, S, H, hd,
+                                            c.kv_heads, window=c.attn_window, sinks=c.attn_sinks)
         if c.pos == "rope":
             ops.rope(dqkv, S, c.d_model + c.kv_heads * hd, hd, c.rope_theta, inverse=True)
         dh1 = ops.linear_dx(dqkv, self._w(self.qkv_w))
@@ -642,7 +686,7 @@ class StageModel:
             elif e == cfg.n_layer + 1:
                 self.layers.append(Head(cfg, self.store, e))
             else:
-                self.layers.append(Block(cfg, self.store, e))
+                self.layers.append(Block(cfg, self.store, e, seed))
 
     @property
     def first(self) -> bool:
@@ -707,15 +751,18 @@ class StageModel:
     def last(self) -> bool:
         return self.hi == self.cfg.n_layer + 2
 
-    def forward(self, inp, targets=None, keep: str = "all"):
-        """F of one microbatch. inp: token ids (first stage) or an Act.
-        keep="all" saves every layer's context for B; keep="inputs" saves only
+    def forward(self, inp, targets=None, keep: str = "all", draw: int | None = None):
+        """F of one microbatch. inp: token ids (first stage) or an Act. draw:
+        the microbatch's number in the run (step * microbatches + mb), which
+        picks its dropout masks; None leaves dropout out. keep="all" saves every layer's context for B; keep="inputs" saves only
         each layer's input (per-layer recompute in B). Returns (output Act or
         loss, per-layer saved state)."""
         saved = []
         h = inp
+        if not self.cfg.dropout:
+            draw = None
         for layer in self.layers:
-            ctx: dict = {}
+            ctx: dict = {} if draw is None else {"draw": draw}
             x_in = h
             if getattr(layer, "is_head", False):
                 h = layer.forward(h, ctx, targets)
@@ -725,7 +772,7 @@ class StageModel:
                 saved.append(("ctx", ctx))
             else:
                 ctx.clear()
-                saved.append(("input", x_in))
+                saved.append(("input", (x_in, draw)))
         return h, saved
 
     def backward(self, saved, dy, wq: list, run_w_inline: bool = False, w_exec=None):
@@ -737,8 +784,11 @@ class StageModel:
         g = dy
         for layer, (kind, obj) in zip(reversed(self.layers), reversed(saved)):
             if kind == "input":
+                x_in, draw = obj
                 ctx: dict = {"_recompute": True}
-                layer.forward(obj, ctx)
+                if draw is not None:
+                    ctx["draw"] = draw
+                layer.forward(x_in, ctx)
             else:
                 ctx = obj
             tasks: list = [] if run_w_inline else wq

@@ -391,6 +391,20 @@ def rope(x, S, ncols, hd, theta, inverse=False):
     return x
 
 
+def rope_rows(x, ncols, hd, cos, sin):
+    """As rope, with a position of its own for every row: cos and sin are the
+    rows' own table entries [rows, hd / 2]."""
+    if _cuda(x):
+        ext().rope(x, x.shape[0], ncols, hd, cos.contiguous(), sin.contiguous(), False)
+        return x
+    v = x[:, :ncols].reshape(x.shape[0], ncols // hd, hd // 2, 2)
+    x1, x2 = v[..., 0].clone(), v[..., 1].clone()
+    v[..., 0] = x1 * cos[:, None] - x2 * sin[:, None]
+    v[..., 1] = x1 * sin[:, None] + x2 * cos[:, None]
+    x[:, :ncols] = v.reshape(x.shape[0], ncols)
+    return x
+
+
 def swiglu_fwd(gu):
     """h = silu(gu[:, :f]) * gu[:, f:]."""
     T, f2 = gu.shape

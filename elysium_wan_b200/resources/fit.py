@@ -59,7 +59,7 @@ def measure(spec, stage: int, device: str = "cpu") -> dict:
                 inp = Act(torch.zeros(T, spec.model.d_model, dtype=dt, device=dev))
                 t = torch.zeros(spec.mb_size, spec.model.seq_len, dtype=torch.long)
             out, st = eng.model.forward(inp, t.to(dev) if eng.last else None,
-                                        keep="inputs" if eng.recompute else "all")
+                                        keep="inputs" if eng.recompute else "all", draw=mb)
             saved.append(st)
         opt.step()
     except torch.cuda.OutOfMemoryError:

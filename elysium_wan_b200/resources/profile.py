@@ -34,7 +34,7 @@ def profile_stage(spec, stage: int, device: str = "cpu", reps: int = 3) -> dict:
             dt = torch.bfloat16 if cuda else torch.float32
             inp = Act(torch.randn(T, spec.model.d_model, device=dev).to(dt))
         t0 = clock()
-        out, st = eng.model.forward(inp, t.to(dev) if eng.last else None)
+        out, st = eng.model.forward(inp, t.to(dev) if eng.last else None, draw=r)
         t1 = clock()
         dy = None if eng.last else torch.randn(T, spec.model.d_model, device=dev).to(
             torch.bfloat16 if cuda else torch.float32)

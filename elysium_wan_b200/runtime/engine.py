@@ -208,7 +208,7 @@ class StageEngine:
                             device=self.device)
             q8 = ops.q8_dtype(s.model.boundary_dtype)
             inp = Act(*ops.quant_q8(z, q8)) if q8 is not None else Act(z)
-        out, st = self.model.forward(inp, x if self.last else None)
+        out, st = self.model.forward(inp, x if self.last else None, draw=0)
         dt = torch.bfloat16 if self.device.type == "cuda" else torch.float32
         dy = None if self.last else torch.zeros((T, s.model.d_model), dtype=dt, device=self.device)
         tasks: list = []
@@ -276,7 +276,8 @@ class StageEngine:
                     act_q[f_mbs[fi]] = comm.irecv_act(f_mbs[fi])
                 tgt = batches[mb][1] if self.last else None
                 mark()
-                out, st = self.model.forward(inp, tgt, keep=keep)
+                out, st = self.model.forward(inp, tgt, keep=keep,
+                                             draw=step * spec.microbatches + mb)
                 saved[mb] = st
                 if self.last:
                     dev_losses.append((mb, out))

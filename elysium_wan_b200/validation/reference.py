@@ -86,7 +86,7 @@ class Oracle:
                     m.store.grad = self.partials[r][owners[r][mb]]
             ctxs, h = [], x
             for m in self.stages:
-                h, c = m.forward(h, t if m.last else None)
+                h, c = m.forward(h, t if m.last else None, draw=step * spec.microbatches + mb)
                 ctxs.append(c)
             loss = h
             dy = None

@@ -1,0 +1,216 @@
+"""Models with an attention window, sinks and residual dropout, and the Decoder.
+
+Would fail if: a mask depended on the cut, the recompute or the replica; a
+gradient left out a mask; a ring's answer differed from the text's own forward;
+or a setting that makes no sense were taken.
+"""
+
+
+import importlib.util
+import os
+
+import pytest
+import torch
+
+from elysium_wan_b200 import ops
+from elysium_wan_b200.models.config import GPTConfig, make_config
+from elysium_wan_b200.models.decode import Decoder
+from elysium_wan_b200.models.gpt import StageModel
+
+TINY = dict(n_layer=2, vocab_size=97, seq_len=40, d_model=64, n_head=4, n_kv_head=2, attn_window=9,
+            attn_sinks=2)
+
+
+def build(device="cpu", preset="llama_tiny", seed=3, **kw):
+    dt = "bf16" if str(device).startswith("cuda") else "fp32"
+    cfg = make_config(preset, **{**dict(compute_dtype=dt, boundary_dtype=dt), **kw})
+    m = StageModel(cfg, (0, cfg.n_entries), device, seed=seed)
+    return cfg, m
+
+
+def step_grads(m, x, y, draw, keep):
+    m.zero_grad()
+    loss, saved = m.forward(x, y, keep=keep, draw=draw)
+    tasks = []
+    m.backward(saved, None, tasks)
+    for t in tasks:
+        t.run()
+    return loss, m.store.grad.clone()
+
+
+def by_name(m):
+    """The gradients in one order on every device (a store's own layout is not)."""
+    return torch.cat([m.store.g(n).double().cpu().reshape(-1) for n in sorted(m.store.names())])
+
+
+def tokens(cfg, B, seed, device="cpu"):
+    g = torch.Generator()
+    g.manual_seed(seed)
+    t = torch.randint(0, cfg.vocab_size, (B, cfg.seq_len + 1), generator=g).to(device)
+    return t[:, :-1].contiguous(), t[:, 1:].contiguous()
+
+
+@pytest.mark.parametrize("bad", [dict(attn_window=0), dict(attn_sinks=2), dict(attn_window=4, attn_sinks=-1),
+                                 dict(dropout=1.0), dict(dropout=-0.1)])
+def test_config_refusals(bad):
+    with pytest.raises(ValueError):
+        make_config("llama_tiny", **bad)
+
+
+def test_old_configs_are_unchanged():
+    cfg = GPTConfig.from_dict(dict(vocab_size=32, n_layer=1))
+    assert cfg.attn_window is None and cfg.attn_sinks == 0 and cfg.dropout == 0.0
+    assert GPTConfig.from_dict(make_config("llama_tiny", attn_window=5, attn_sinks=1,
+                                           dropout=0.1).to_dict()).attn_window == 5
+
+
+@pytest.mark.parametrize("preset,kw", [("llama_tiny", {**TINY, "dropout": 0.2}),
+                                       ("toy", dict(n_layer=2, dropout=0.3)),
+                                       ("moe_tiny", dict(n_layer=1, seq_len=32, vocab_size=64, dropout=0.1))])
+def test_host_recompute_and_draws(preset, kw):
+    cfg, m = build(preset=preset, **kw)
+    x, y = tokens(cfg, 2, 0)
+    l0, g0 = step_grads(m, x, y, 7, "all")
+    l1, g1 = step_grads(m, x, y, 7, "inputs")
+    assert torch.equal(l0, l1) and torch.equal(g0, g1)
+    l2, _ = step_grads(m, x, y, 8, "all")  # another microbatch, other masks
+    l3, _ = step_grads(m, x, y, None, "all")
+    assert not torch.equal(l0, l2) and not torch.equal(l0, l3)
+
+
+def test_host_gradient_against_differences():
+    """The loss of one draw is a smooth function of the parameters: its
+    difference quotient is the gradient (fp32: 2e-3 of the largest one)."""
+    cfg, m = build(**{**TINY, "dropout": 0.25})
+    x, y = tokens(cfg, 2, 1)
+    _, g = step_grads(m, x, y, 5, "all")
+    gen = torch.Generator()
+    gen.manual_seed(0)
+    for _ in range(3):
+        u = torch.randn(g.shape, generator=gen)
+        u /= u.norm()
+        base, f, h = m.store.master.clone(), [], 3e-2
+        for sign in (1, -1):
+            m.store.master.copy_(base + sign * h * u)
+            f.append(float(m.forward(x, y, draw=5)[0]))
+        m.store.master.copy_(base)
+        assert abs((f[0] - f[1]) / (2 * h) - float((g * u).sum())) < 2e-3 * float(g.norm())
+
+
+def test_host_pipeline_equals_the_oracle(tmp_path):
+    from elysium_wan_b200.launch.local import run_and_compare
+    from elysium_wan_b200.runtime.spec import JobSpec
+
+    cfg = make_config("llama_tiny", **{**TINY, "n_layer": 3, "dropout": 0.1})
+    spec = JobSpec(model=cfg, stages=2, microbatches=4, mb_size=2, steps=2, backend="gloo",
+                   out_dir=str(tmp_path))
+    r = run_and_compare(spec.finalize(), timeout=240)
+    assert r["ok"], r
+
+
+def check_decoder(device, tol, **kw):
+    cfg, m = build(device, **kw)
+    dec = Decoder(m, logit_rows=24)
+    B = 3
+    x, y = tokens(cfg, B, 2, device)
+    y = torch.where(torch.arange(cfg.seq_len, device=device) % 5 == 4, -1, y)
+    r = dec.score(x, y, top=4)
+    lg = dec._logits_of(dec._final_norm(*(lambda h: (h.x, h.scale))(dec.hidden(x))))[:, :cfg.vocab_size]
+    lp = torch.log_softmax(lg.double(), 1)
+    want = torch.where(y.reshape(-1) >= 0, lp.gather(1, y.reshape(-1).clamp(min=0)[:, None])[:, 0], 0.0)
+    assert float((r.logp - want).abs().max()) < 1e-4
+    assert torch.equal(r.top_ids[:, 0], lg.argmax(1))
+    # the same text token by token, from prompts of three lengths
+    lengths = torch.tensor([0, 5, 21], dtype=torch.int32, device=device)
+    caches = dec.new_caches(B)
+    pos = dec.prefill(x, lengths, caches)
+    lp = lp.view(B, cfg.seq_len, -1)
+    for i in range(cfg.seq_len):
+        live = pos < cfg.seq_len
+        at = pos.clamp(max=cfg.seq_len - 1)
+        out = dec.step(x.gather(1, at[:, None])[:, 0], torch.where(live, pos, -1), caches, top=4)
+        for b in range(B):
+            if live[b]:
+                ref = lp[b, at[b]]
+                assert float((out.top_logp[b].double() - ref[out.top_ids[b]]).abs().max()) < tol
+        pos = pos + 1
+    return cfg, dec, caches, pos
+
+
+def test_host_decoder():
+    for kw in (dict(TINY), dict(preset="toy", n_layer=2, attn_window=6), dict(TINY, attn_window=None, attn_sinks=0)):
+        check_decoder("cpu", 1e-4, **kw)
+
+
+def test_host_decoder_past_the_text_and_refusals():
+    cfg, dec, caches, pos = check_decoder("cpu", 1e-4, **TINY)
+    for _ in range(30):  # rotary positions and the ring go on
+        out = dec.step(torch.zeros(3, dtype=torch.int64), pos, caches)
+        pos = pos + 1
+    assert torch.isfinite(out.entropy).all()
+    cfg, dec, caches, pos = check_decoder("cpu", 1e-4, preset="toy", n_layer=2, attn_window=6)
+    with pytest.raises(ValueError, match="seq_len"):
+        dec.step(torch.zeros(3, dtype=torch.int64), torch.full((3,), cfg.seq_len), caches)
+    with pytest.raises(ValueError, match="texts come as"):
+        dec.hidden(torch.zeros(1, 5, dtype=torch.int64))
+    c = make_config("moe_tiny")
+    with pytest.raises(ValueError, match="dense"):
+        Decoder(StageModel(c, (0, c.n_entries), "cpu", seed=0))
+
+
+# ----------------------------------------------------------------------------- GPU
+GPU = dict(n_layer=2, vocab_size=211, seq_len=200, d_model=256, n_head=4, n_kv_head=2, attn_window=50,
+           attn_sinks=3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("boundary", ["bf16", "fp16", "fp8_e4m3_b128"])
+def test_gpu_recompute_and_host_agree(cuda, boundary):
+    """Bitwise equal with and without recompute; near the host path, which draws
+    the same masks (a wrong one would move the loss by far more than bf16 does)."""
+    kw = dict(GPU, dropout=0.2, boundary_dtype=boundary)
+    cfg, m = build(cuda, **kw)
+    x, y = tokens(cfg, 2, 4, cuda)
+    l0, g0 = step_grads(m, x, y, 3, "all")
+    l1, g1 = step_grads(m, x, y, 3, "inputs")
+    assert torch.equal(l0, l1) and torch.equal(g0, g1)
+    g0 = by_name(m)
+    hc, h = build("cpu", **{**kw, "compute_dtype": "fp32"})
+    for n in h.store.names():  # initial values are drawn on each device by itself
+        h.store.p(n).copy_(m.store.p(n))
+    lh, _ = step_grads(h, x.cpu(), y.cpu(), 3, "all")
+    gh = by_name(h)
+    assert abs(float(l0) - float(lh)) < 0.02
+    cos = torch.nn.functional.cosine_similarity(g0, gh, 0)
+    assert float(cos) > 0.98
+    step_grads(h, x.cpu(), y.cpu(), 4, "all")
+    other = torch.nn.functional.cosine_similarity(gh, by_name(h), 0)
+    assert float(other) < float(cos) - 0.005
+
+
+@pytest.mark.gpu
+def test_gpu_decoder(cuda):
+    # logits of size 1 from bf16 activations in another order of sums: 2^-8 of
+    # each of a few hundred terms, taken together under 0.06
+    cfg, dec, caches, pos = check_decoder(cuda, 0.06, **GPU)
+    for _ in range(5):
+        out = dec.step(torch.zeros(3, dtype=torch.int64, device=cuda), pos, caches, top=3)
+        pos = pos + 1
+    assert torch.isfinite(out.entropy).all() and ops.ext().status_record()[0] == 0
+
+
+def example():
+    p = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "long_text", "run.py")
+    spec = importlib.util.spec_from_file_location("long_text_example", p)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    return mod
+
+
+@pytest.mark.gpu
+def test_gpu_example(cuda):
+    assert example().main(["--device", "cuda:0", "--steps", "30", "--answer", "20"]) == 0
+
+
+def test_host_example():
+    assert example().main(["--device", "cpu", "--steps", "12", "--answer", "8"]) == 0

@@ -530,11 +530,13 @@ __global__ void __launch_bounds__(kWbThreads, 1)
       int i = a.i0;
       for (int t = 0; t < a.steps; ++t, ++tn) {
         const int s = tn & 1;
-        ok = warp_wait(sfull, tn & 1, status, kStatusTimeoutTmemFull) &&
-             warp_wait(&qfull[s], (tn >> 1) & 1, status, kStatusTimeoutSmemFull);
+        // the statistics, and this step's mask, before the scores are there
+        ok = warp_wait(&qfull[s], (tn >> 1) & 1, status, kStatusTimeoutSmemFull);
         if (!ok) break;
-        tc_fence_after();
         const uint32_t stat = smem_u32(smem + L::kStat) + s * 1024 + g * 256;
+        f32x2 st[16];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) lds4(stat + e * 16, st[2 * e], st[2 * e + 1]);
         // queries of this half that see key kpos: from kpos on, below kpos + window
         uint32_t vis[2] = {0xffffffffu, 0xffffffffu};
         const bool whole = i * 128 >= a.k0 + 127 && a.k0 + 128 <= a.n &&
@@ -547,16 +549,19 @@ __global__ void __launch_bounds__(kWbThreads, 1)
             if (kpos >= plan.sinks) vis[c] &= bits_below(kpos + plan.window - c0);
           }
         }
+        ok = warp_wait(sfull, tn & 1, status, kStatusTimeoutTmemFull);
+        if (!ok) break;
+        tc_fence_after();
         uint32_t v[64];
         tmem_ld32(half, v);
         tmem_ld32(half + 32, v + 32);
+        tmem_wait_ld();
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          f32x2 nl[16];
+          weights32(v + 32 * c, scale2, [&](int e) { return st[e]; });
+          // those of the next 32 columns, or the first -D
 #pragma unroll
-          for (int e = 0; e < 8; ++e) lds4(stat + c * 128 + e * 16, nl[2 * e], nl[2 * e + 1]);
-          if (c == 0) tmem_wait_ld();
-          weights32(v + 32 * c, scale2, [&](int e) { return nl[e]; });
+          for (int e = 0; e < 8; ++e) lds4(stat + (c ? 512 : 128) + e * 16, st[2 * e], st[2 * e + 1]);
           if (!whole) clear32(v + 32 * c, vis[c]);
           store32(half + c * 16, v + 32 * c);
           tmem_wait_st();
@@ -570,12 +575,13 @@ __global__ void __launch_bounds__(kWbThreads, 1)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t d[32];
-          f32x2 nd[16];
           tmem_ld32(half + 128 + c * 32, d);
+          if (c == 1) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) lds4(stat + 512 + c * 128 + e * 16, nd[2 * e], nd[2 * e + 1]);
+            for (int e = 0; e < 8; ++e) lds4(stat + 640 + e * 16, st[2 * e], st[2 * e + 1]);
+          }
           tmem_wait_ld();
-          grads32(d, v + 32 * c, [&](int e) { return nd[e]; });
+          grads32(d, v + 32 * c, [&](int e) { return st[e]; });
           if (!whole) clear32(d, vis[c]);  // dP of a key past the length may be NaN
           store32(half + 128 + c * 16, d);
         }

@@ -113,42 +113,78 @@ __device__ __forceinline__ int next_block_read(const void* answer) {
 }
 
 // The items of a CTA: its own block index, then those of blocks that it takes
-// over (next_block_ask), one asked for ahead. Every warp that works on items
-// walks them with one of these.
-struct BlockQueue {
-  void* answer;
-  uint64_t *full, *empty;
+// over (next_block_ask), one asked for ahead. The asking warp works out what the
+// roles have to know of an item and leaves it in shared memory: each role doing
+// so for itself (a handful of divisions) stood between two items.
+template <typename Item>
+struct ItemQueue {
+  static constexpr int kWords = sizeof(Item) / 4;
+  static_assert(sizeof(Item) % 4 == 0 && kWords < 32, "one word a lane");
+  uint32_t slot;          // shared memory: the item, then 1, or 0 for none left
+  void* answer;           // 16 bytes
+  uint64_t *asked, *full, *empty;
   int seen = 0;
-  // The next item after `w`; -1: none left (or a wait ran out).
-  __device__ __forceinline__ int next(int* status, int lane) {
-    if (!warp_wait(full, seen & 1, status, kStatusTimeoutSmemFull)) return -1;
-    const int w = __shfl_sync(0xffffffffu, next_block_read(answer), 0);
+
+  // The next item; false: none left (or a wait ran out). `also` reads what else
+  // the asking warp left for this item.
+  template <typename F>
+  __device__ __forceinline__ bool next(Item& a, int* status, int lane, F also) {
+    if (!warp_wait(full, seen & 1, status, kStatusTimeoutSmemFull)) return false;
     ++seen;
-    fence_proxy_async_smem();  // read before the next answer is written over it
-    __syncwarp();
+    uint32_t v = 0u, words[kWords];
+    if (lane <= kWords) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(slot + lane * 4));
+    also();
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) words[i] = __shfl_sync(0xffffffffu, v, i);
+    const bool some = __shfl_sync(0xffffffffu, v, kWords) != 0u;
+    __syncwarp();  // every lane has read
     if (lane == 0) mbar_arrive(empty);
-    return w;
+    __builtin_memcpy(&a, words, sizeof(Item));
+    return some;
+  }
+  __device__ __forceinline__ bool next(Item& a, int* status, int lane) {
+    return next(a, status, lane, [] {});
+  }
+
+  // The asking warp: one question at a time, once every role has taken the item
+  // before (`empty` counts the warps that walk the queue). make(w): the item of
+  // block w, and whatever `also` reads.
+  template <typename F>
+  __device__ __forceinline__ void ask(int* status, int lane, F make) {
+    int w = blockIdx.x;
+    for (int i = 0;; ++i) {
+      if (i > 0) {
+        // a wait that ran out: nothing is asked for, and the roles' own waits end
+        if (!warp_wait(empty, (i - 1) & 1, status, kStatusTimeoutSmemEmpty)) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(asked, 16);
+          next_block_ask(answer, asked);
+        }
+        __syncwarp();
+        if (!warp_wait(asked, (i - 1) & 1, status, kStatusTimeoutSmemFull)) {
+          mbar_wait(asked, (i - 1) & 1, nullptr, kStatusTimeoutDrain);  // the answer must land
+          break;
+        }
+        w = __shfl_sync(0xffffffffu, next_block_read(answer), 0);
+        fence_proxy_async_smem();  // read before the next answer is written over it
+      }
+      uint32_t words[kWords + 1] = {};
+      if (w >= 0) {
+        const Item a = make(w);
+        __builtin_memcpy(words, &a, sizeof(Item));
+        words[kWords] = 1u;
+      }
+      if (lane == 0) {
+#pragma unroll
+        for (int k = 0; k <= kWords; ++k)
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(slot + k * 4), "r"(words[k]) : "memory");
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(full);
+      if (w < 0) break;
+    }
   }
 };
-
-// The asking warp: one question at a time, once every role has taken the answer
-// before (`empty` counts the warps that walk the queue).
-__device__ __forceinline__ void ask_blocks(const BlockQueue& q, int* status, int lane) {
-  for (int i = 0;; ++i) {
-    // a wait that ran out: nothing is asked for, and the roles' own waits end
-    if (!warp_wait(q.empty, (i & 1) ^ 1, status, kStatusTimeoutSmemEmpty)) break;
-    if (lane == 0) {
-      mbar_arrive_expect_tx(q.full, 16);
-      next_block_ask(q.answer, q.full);
-    }
-    __syncwarp();
-    if (!warp_wait(q.full, i & 1, status, kStatusTimeoutSmemFull)) {
-      mbar_wait(q.full, i & 1, nullptr, kStatusTimeoutDrain);  // the answer must land
-      break;
-    }
-    if (__shfl_sync(0xffffffffu, next_block_read(q.answer), 0) < 0) break;
-  }
-}
 
 template <int N>
 __device__ __forceinline__ void reg_dec() {
@@ -177,6 +213,7 @@ __device__ __forceinline__ void mask32(uint32_t* v, uint32_t bits) {
 // them and positions stay inside 32 bits.
 struct TileList {
   int ns, w0, e;
+  TileList() = default;
   __device__ __forceinline__ TileList(int q0, int q1, int window, int sinks) {
     w0 = max(0, q0 - window + 1) >> 7;
     e = q1 >> 7;

@@ -63,9 +63,9 @@ struct WaItem {
   int live;   // subtiles with a row below the length
   int tiles;  // key tiles of the item
   TileList all, sub0, sub1;
+  WaItem() = default;
   __device__ __forceinline__ WaItem(int w, int B, int H, int rep, int S, int blocks, int window, int sinks,
-                                    const int* lengths)
-      : all(0, 0, 1, 0), sub0(0, 0, 1, 0), sub1(0, 0, 1, 0) {
+                                    const int* lengths) {
     h = w % H;
     w /= H;
     b = w % B;
@@ -132,9 +132,10 @@ __global__ void __launch_bounds__(kWaThreads, 1)
   uint64_t* landed = bars + 22;   // a V tile that the producer clears
   uint64_t* drain = bars + 23;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
-  uint64_t* wfull = bars + 26;   // the next item's index
+  uint64_t* wfull = bars + 26;   // the next item
   uint64_t* wempty = bars + 27;  // read by the producer, the MMA warp and the softmax warps
   uint64_t* answer = bars + 28;  // [2]
+  uint64_t* asked = bars + 30;
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rep = H / Hkv, blocks = (S + 255) / 256;
@@ -156,6 +157,7 @@ __global__ void __launch_bounds__(kWaThreads, 1)
     mbar_init(landed, 1);
     mbar_init(drain, 1);
     mbar_init(wfull, 1);
+    mbar_init(asked, 1);
     mbar_init(wempty, 10);
     fence_mbar_init();
     tma_prefetch_desc(&map);
@@ -169,17 +171,16 @@ __global__ void __launch_bounds__(kWaThreads, 1)
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
-  BlockQueue queue{answer, wfull, wempty};
+  ItemQueue<WaItem> queue{smem_u32(smem + L::kBar) + 256, answer, asked, wfull, wempty};
   if (warp < 4) {
     reg_dec<kWaRegsIssue>();
     if (warp == 2) {
-      ask_blocks(queue, status, lane);
+      queue.ask(status, lane, [&](int w) { return WaItem(w, B, H, rep, S, blocks, window, sinks, lengths); });
     } else if (warp == 0) {
       bool ok = true;
       int kv = 0, qn[2] = {0, 0}, cleared = 0;  // K / V tiles, Q subtiles, cleared tiles so far
       int last_cleared = -1;                    // the last of them, as a number of kv
-      for (int w = blockIdx.x; w >= 0 && ok; w = queue.next(status, lane)) {
-        const WaItem a(w, B, H, rep, S, blocks, window, sinks, lengths);
+      for (WaItem a; ok && queue.next(a, status, lane);) {
         // The V tile that holds row n of a sequence shorter than S is cleared
         // from that row on before it is handed over.
         const int clear = (a.n < S && (a.n & 127)) ? a.n >> 7 : -1;
@@ -265,10 +266,10 @@ __global__ void __launch_bounds__(kWaThreads, 1)
       bool begin[2] = {false, false};  // begins O_t,
       bool end[2] = {false, false};    // ends it
       bool held = false;               // the V tile before is still needed
-      int w = blockIdx.x;
       while (ok) {
-        const WaItem a(max(w, 0), B, H, rep, S, blocks, window, sinks, lengths);
-        const int tiles = w >= 0 ? a.tiles : 0;
+        WaItem a;
+        const bool some = queue.next(a, status, lane);
+        const int tiles = some ? a.tiles : 0;
         bool begun[2] = {false, false};
         for (int k = 0; k < max(tiles, 1) && ok; ++k) {
           const bool more = k < tiles;
@@ -334,8 +335,7 @@ __global__ void __launch_bounds__(kWaThreads, 1)
             ++kv;
           }
         }
-        if (w < 0) break;
-        w = queue.next(status, lane);
+        if (!some) break;
       }
       umma_commit_by(lead, drain);
       mbar_wait(drain, 0, nullptr, kStatusTimeoutDrain);
@@ -352,8 +352,7 @@ __global__ void __launch_bounds__(kWaThreads, 1)
     bool ok = true;
     int sn = 0;     // tiles so far: parity of S_t
     int items = 0;  // live items so far: parity of O_t
-    for (int w = blockIdx.x; w >= 0; w = ok ? queue.next(status, lane) : -1) {
-      const WaItem a(w, B, H, rep, S, blocks, window, sinks, lengths);
+    for (WaItem a; ok && queue.next(a, status, lane);) {
       const TileList& sub = t ? a.sub1 : a.sub0;
       const int mine = t < a.live ? sub.count() : 0;
       const int first = a.q0 + t * 128, row = first + r;

@@ -165,7 +165,8 @@ struct KvLayout {
 
 struct KvItem {
   int hk, b, kt, part, n, k0, i0, nqs, steps;
-  bool split;
+  int split;
+  KvItem() = default;
   __device__ __forceinline__ KvItem(int w, const KvPlan& plan, int B, int S, int Hkv, int rep, const int* lengths) {
     hk = w % Hkv;
     w /= Hkv;
@@ -227,6 +228,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
   uint64_t* answer = bars + 22;  // [2], 16-byte aligned
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
   uint64_t* pfull2 = bars + 25;
+  uint64_t* asked = bars + 26;
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rep = H / Hkv;
@@ -242,6 +244,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
     mbar_init(landed, 1);
     mbar_init(drain, 1);
     mbar_init(wfull, 1);
+    mbar_init(asked, 1);
     mbar_init(wempty, kWbWalkers);
     fence_mbar_init();
     tma_prefetch_desc(&map);
@@ -255,20 +258,19 @@ __global__ void __launch_bounds__(kWbThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-  BlockQueue queue{answer, wfull, wempty};
+  ItemQueue<KvItem> queue{smem_u32(smem + L::kBar) + 256, answer, asked, wfull, wempty};
 
   if (warp < 4) {
     reg_dec<kWbRegsIssue>();
     if (warp == 2) {
-      ask_blocks(queue, status, lane);
+      queue.ask(status, lane, [&](int w) { return KvItem(w, plan, B, S, Hkv, rep, lengths); });
     } else if (warp == 0) {
       bool ok = true;
       int items = 0, tn = 0, cleared = 0;
       int kn = 0, vn = 0;              // K and V tiles issued
       int qn = 0, gn = 0;              // Q and dO tiles issued on their own barriers
       int last_cleared = -1;           // the last step whose tiles came over `landed`
-      for (int w = blockIdx.x; w >= 0 && ok; w = ok ? queue.next(status, lane) : -1) {
-        const KvItem a(w, plan, B, S, Hkv, rep, lengths);
+      for (KvItem a; ok && queue.next(a, status, lane);) {
         const int clear = (a.n < S && (a.n & 127)) ? a.n >> 7 : -1;  // the tile that holds row n
         for (int t = 0; t < a.steps && ok; ++t) {
           const int s = tn & 1;
@@ -371,10 +373,10 @@ __global__ void __launch_bounds__(kWbThreads, 1)
       int items = 0, tn = 0, accs = 0;
       // the step before: to be finished, the first or last of its block
       bool held = false, first = false, last = false;
-      int w = blockIdx.x;
       while (ok) {
-        const KvItem a(max(w, 0), plan, B, S, Hkv, rep, lengths);
-        const int steps = w >= 0 ? a.steps : 0;
+        KvItem a;
+        const bool some = queue.next(a, status, lane);
+        const int steps = some ? a.steps : 0;
         // a block without work only lets the step before through
         for (int t = 0; t < max(steps, 1) && ok; ++t) {
           const bool more = t < steps;
@@ -449,9 +451,8 @@ __global__ void __launch_bounds__(kWbThreads, 1)
           last = t == steps - 1;
           if (more) ++tn;
         }
-        if (w < 0) break;
+        if (!some) break;
         if (steps > 0) ++items;
-        w = queue.next(status, lane);
       }
       umma_commit_by(lead, drain);
       mbar_wait(drain, 0, nullptr, kStatusTimeoutDrain);
@@ -465,8 +466,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
     const int64_t ldq = static_cast<int64_t>(H + 2 * Hkv) * HD;
     bool ok = true;
     int items = 0;
-    for (int w = blockIdx.x; w >= 0 && ok; w = ok ? queue.next(status, lane) : -1) {
-      const KvItem a(w, plan, B, S, Hkv, rep, lengths);
+    for (KvItem a; ok && queue.next(a, status, lane);) {
       const bool some = a.steps > 0;
       if (some) {
         ok = warp_wait(accfull, items & 1, status, kStatusTimeoutTmemFull);
@@ -524,8 +524,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
     const f32x2 scale2 = pair2(scale_log2, scale_log2);
     bool ok = true;
     int tn = 0;
-    for (int w = blockIdx.x; w >= 0 && ok; w = ok ? queue.next(status, lane) : -1) {
-      const KvItem a(w, plan, B, S, Hkv, rep, lengths);
+    for (KvItem a; ok && queue.next(a, status, lane);) {
       const int kpos = a.k0 + r;
       int i = a.i0;
       for (int t = 0; t < a.steps; ++t, ++tn) {
@@ -649,16 +648,16 @@ struct DqLayout {
   static constexpr int kChunks = HeadChunks<HD>::kCount;
   static constexpr uint32_t kTile = kChunks * kWaChunk;
   static constexpr uint32_t kQ = 0, kO = kTile, kK = 2 * kTile, kV = 5 * kTile;
-  static constexpr uint32_t kStage = 6 * kTile, kBar = kStage + 4 * 4096;
+  static constexpr uint32_t kStage = 6 * kTile, kStat = kStage + 4 * 4096, kBar = kStat + 1024;
   static constexpr int kSmem = static_cast<int>(kBar) + 512 + 1024;
 };
 
 struct DqItem {
   int h, b, hk, q0, n, tiles;
   TileList list;
+  DqItem() = default;
   __device__ __forceinline__ DqItem(int w, int B, int H, int rep, int S, int blocks, int window, int sinks,
-                                    const int* lengths)
-      : list(0, 0, 1, 0) {
+                                    const int* lengths) {
     h = w % H;
     w /= H;
     b = w % B;
@@ -690,7 +689,6 @@ __global__ void __launch_bounds__(kWbThreads, 1)
   uint64_t* kfull = bars + 4;   // [3]
   uint64_t* kempty = bars + 7;  // [3]
   uint64_t* vfull = bars + 10;
-  uint64_t* vempty = bars + 11;
   uint64_t* sfull = bars + 12;  // [2]
   uint64_t* dpfull = bars + 14;
   uint64_t* dpfree = bars + 15;
@@ -703,6 +701,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
   uint64_t* wempty = bars + 23;
   uint64_t* answer = bars + 24;  // [2], 16-byte aligned
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 26);
+  uint64_t* asked = bars + 27;
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rep = H / Hkv, blocks = Sp / 128;
@@ -716,6 +715,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
     mbar_init(landed, 1);
     mbar_init(drain, 1);
     mbar_init(wfull, 1);
+    mbar_init(asked, 1);
     mbar_init(wempty, kWbWalkers);
     fence_mbar_init();
     tma_prefetch_desc(&map);
@@ -729,17 +729,26 @@ __global__ void __launch_bounds__(kWbThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-  BlockQueue queue{answer, wfull, wempty};
+  ItemQueue<DqItem> queue{smem_u32(smem + L::kBar) + 256, answer, asked, wfull, wempty};
 
   if (warp < 4) {
     reg_dec<kWbRegsIssue>();
     if (warp == 2) {
-      ask_blocks(queue, status, lane);
+      queue.ask(status, lane, [&](int w) {
+        const DqItem a(w, B, H, rep, S, blocks, window, sinks, lengths);
+        const int64_t at = (static_cast<int64_t>(a.b) * H + a.h) * Sp + a.q0 + lane;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // padded rows: -inf, 0
+          const uint32_t to = smem_u32(smem + L::kStat) + (i * 32 + lane) * 8;
+          asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(NL[at + 32 * i]), "f"(ND[at + 32 * i])
+                       : "memory");
+        }
+        return a;
+      });
     } else if (warp == 0) {
       bool ok = true;
       int items = 0, kv = 0, vn = 0, gn = 0, qn = 0, cleared = 0, last_cleared = -1;
-      for (int w = blockIdx.x; w >= 0 && ok; w = ok ? queue.next(status, lane) : -1) {
-        const DqItem a(w, B, H, rep, S, blocks, window, sinks, lengths);
+      for (DqItem a; ok && queue.next(a, status, lane);) {
         const int clear = (a.n < S && (a.n & 127)) ? a.n >> 7 : -1;  // the tile that holds row n
         for (int k = 0; k < a.tiles && ok; ++k) {
           const int j = a.list.tile(k), s = kv % 3;
@@ -786,7 +795,8 @@ __global__ void __launch_bounds__(kWbThreads, 1)
             }
             ++gn;
           }
-          ok = ok && warp_wait(vempty, (vn & 1) ^ 1, status, kStatusTimeoutSmemEmpty);
+          // the dP before has read the V before
+          ok = ok && warp_wait(dpfull, (vn & 1) ^ 1, status, kStatusTimeoutSmemEmpty);
           if (!ok) break;
           if (lane == 0) {
             mbar_arrive_expect_tx(vfull, L::kTile);
@@ -819,10 +829,10 @@ __global__ void __launch_bounds__(kWbThreads, 1)
       int dpn = 0, dqn = 0;  // tiles whose dP, whose dQ was issued
       // the tiles one and two before: there, the first or last of their block
       bool on1 = false, first1 = false, last1 = false, on2 = false, first2 = false, last2 = false;
-      int w = blockIdx.x;
       while (ok) {
-        const DqItem a(max(w, 0), B, H, rep, S, blocks, window, sinks, lengths);
-        const int tiles = w >= 0 ? a.tiles : 0;
+        DqItem a;
+        const bool some = queue.next(a, status, lane);
+        const int tiles = some ? a.tiles : 0;
         // A block lets both tiles before it through, whatever it has itself: the
         // epilogue takes no further block before them, and so none is asked for.
         for (int k = 0; k < max(tiles, 2) && ok; ++k) {
@@ -843,7 +853,6 @@ __global__ void __launch_bounds__(kWbThreads, 1)
                   umma_ss(lead, tmem + 256, desc_at(g_desc, c * kWaChunk + kk * 32),
                           desc_at(v_desc, c * kWaChunk + kk * 32), IS, (c > 0 || kk > 0) ? 1u : 0u);
               umma_commit_by(lead, dpfull);
-              umma_commit_by(lead, vempty);
               if (last1) umma_commit_by(lead, gempty);
             }
             ++dpn;
@@ -890,9 +899,8 @@ __global__ void __launch_bounds__(kWbThreads, 1)
           first1 = k == 0;
           last1 = k == tiles - 1;
         }
-        if (w < 0) break;
+        if (!some) break;
         if (tiles > 0) ++items;
-        w = queue.next(status, lane);
       }
       umma_commit_by(lead, drain);
       mbar_wait(drain, 0, nullptr, kStatusTimeoutDrain);
@@ -906,8 +914,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
     const int64_t ldq = static_cast<int64_t>(H + 2 * Hkv) * HD;
     bool ok = true;
     int items = 0;
-    for (int w = blockIdx.x; w >= 0 && ok; w = ok ? queue.next(status, lane) : -1) {
-      const DqItem a(w, B, H, rep, S, blocks, window, sinks, lengths);
+    for (DqItem a; ok && queue.next(a, status, lane);) {
       const bool some = a.tiles > 0;
       if (some) {
         ok = warp_wait(accfull, items & 1, status, kStatusTimeoutTmemFull);
@@ -951,11 +958,12 @@ __global__ void __launch_bounds__(kWbThreads, 1)
     const f32x2 scale2 = pair2(scale_log2, scale_log2);
     bool ok = true;
     int tn = 0;
-    for (int w = blockIdx.x; w >= 0 && ok; w = ok ? queue.next(status, lane) : -1) {
-      const DqItem a(w, B, H, rep, S, blocks, window, sinks, lengths);
+    float nl, nd;
+    auto stats = [&] {
+      asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(nl), "=f"(nd) : "r"(smem_u32(smem + L::kStat) + r * 8));
+    };
+    for (DqItem a; ok && queue.next(a, status, lane, stats);) {
       const int row = a.q0 + r;
-      const int64_t at = (static_cast<int64_t>(a.b) * H + a.h) * Sp + row;
-      const float nl = NL[at], nd = ND[at];  // padded rows: -inf, 0
       const f32x2 nl2 = pair2(nl, nl), nd2 = pair2(nd, nd);
       for (int k = 0; k < a.tiles; ++k, ++tn) {
         const uint32_t s_t = half + (tn & 1) * 128;

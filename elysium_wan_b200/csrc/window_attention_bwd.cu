@@ -475,8 +475,11 @@ __global__ void __launch_bounds__(kWbThreads, 1)
         tc_fence_after();
       }
       const int row0 = a.k0 + wq * 32;
+      // of a sinks' tile: sums of parts where these rows have a sink; else only the
+      // first part has anything, their gradients
+      const bool sums = a.split && row0 < plan.sinks, grads = !a.split || (a.part == 0 && !sums);
       float* sum = part_ws;
-      if (a.split)
+      if (sums)
         sum += ((((static_cast<size_t>(a.b) * Hkv + a.hk) * plan.sink_tiles + a.kt) * plan.parts + a.part) * 128 +
                 wq * 32 + lane) * (2 * HD);
 #pragma unroll 1
@@ -496,7 +499,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
 #pragma unroll
               for (int k = 0; k < 16; ++k) v[k] = 0u;
             }
-            if (a.split && 2 * e < C::units(c)) {
+            if (sums && 2 * e < C::units(c)) {
 #pragma unroll
               for (int k = 0; k < 4; ++k)
                 *reinterpret_cast<uint4*>(sum + z * HD + c * 64 + e * 16 + 4 * k) =
@@ -511,7 +514,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(accfree);
           }
-          if (!a.split) store_rows(y, stage, out + c * 64, ldq, C::units(c), S - row0, lane);
+          if (grads) store_rows(y, stage, out + c * 64, ldq, C::units(c), S - row0, lane);
         }
       }
     }
@@ -601,27 +604,26 @@ __global__ void __launch_bounds__(kWbThreads, 1)
   }
 }
 
-// dK, dV of the sinks' tiles: the parts' sums, added in order. One thread per
-// four columns of a row ([dV | dK], 2 HD wide).
+// dK, dV of the sinks and what shares their 32 rows: the parts' sums, added in
+// order. One thread per four columns of a row ([dV | dK], 2 HD wide).
 __global__ void __launch_bounds__(256)
     window_sinks_kernel(const float* __restrict__ ws, __nv_bfloat16* __restrict__ dqkv, int S, int H,
-                        int Hkv, int HD, int sink_tiles, int parts, float scale, int64_t units) {
+                        int Hkv, int HD, int rows, int sink_tiles, int parts, float scale,
+                        int64_t units) {
   const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (t >= units) return;
   const int per = 2 * HD / 4;
   const int c = static_cast<int>(t % per) * 4;
-  int64_t rest = t / per;
-  const int r = static_cast<int>(rest % 128);
-  rest /= 128;  // (b, hk, kt)
-  const int kt = static_cast<int>(rest % sink_tiles);
-  const int64_t bh = rest / sink_tiles;
+  const int64_t rest = t / per;
+  const int kpos = static_cast<int>(rest % rows);
+  const int64_t bh = rest / rows;
   const int hk = static_cast<int>(bh % Hkv);
   const int64_t b = bh / Hkv;
-  const int kpos = kt * 128 + r;
   if (kpos >= S) return;
+  const float* sums = ws + ((bh * sink_tiles + kpos / 128) * parts * 128 + kpos % 128) * (2 * HD) + c;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int p = 0; p < parts; ++p) {
-    const float4 v = *reinterpret_cast<const float4*>(ws + ((rest * parts + p) * 128 + r) * (2 * HD) + c);
+    const float4 v = *reinterpret_cast<const float4*>(sums + static_cast<int64_t>(p) * 128 * 2 * HD);
     a.x += v.x;
     a.y += v.y;
     a.z += v.z;
@@ -1070,9 +1072,10 @@ int launch_bwd(const WindowAttnBwdArgs& a, cudaStream_t stream) {
   window_dkdv_kernel<HD><<<static_cast<unsigned>(kv_blocks), kWbThreads, KvLayout<HD>::kSmem, stream>>>(
       m, mdo, NL, ND, f.lengths, a.dqkv, parts, f.B, f.S, Sp, f.H, f.Hkv, plan, sl2, f.scale, f.status);
   if (plan.parts > 1) {
-    const int64_t t = static_cast<int64_t>(f.B) * f.Hkv * plan.sink_tiles * 128 * (2 * HD / 4);
+    const int rows = (plan.sinks + 31) / 32 * 32;
+    const int64_t t = static_cast<int64_t>(f.B) * f.Hkv * rows * (2 * HD / 4);
     window_sinks_kernel<<<static_cast<unsigned>((t + 255) / 256), 256, 0, stream>>>(
-        parts, a.dqkv, f.S, f.H, f.Hkv, HD, plan.sink_tiles, plan.parts, f.scale, t);
+        parts, a.dqkv, f.S, f.H, f.Hkv, HD, rows, plan.sink_tiles, plan.parts, f.scale, t);
   }
   window_dq_kernel<HD><<<static_cast<unsigned>(q_blocks), kWbThreads, DqLayout<HD>::kSmem, stream>>>(
       m, mdo, NL, ND, f.lengths, a.dqkv, f.B, f.S, Sp, f.H, f.Hkv, plan.window, plan.sinks, sl2, f.scale, f.status);

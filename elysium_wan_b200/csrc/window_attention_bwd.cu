@@ -44,6 +44,7 @@ __global__ void __launch_bounds__(256)
                       float* __restrict__ NL, float* __restrict__ ND, int S, int Sp, int H, int HD,
                       int64_t units) {
   constexpr int kHeads = 4;
+  grid_release();
   const int half = threadIdx.x >> 4, l = threadIdx.x & 15;
   const int64_t u = static_cast<int64_t>(blockIdx.x) * 16 + half;  // (b, s, group of heads)
   if (u >= units) return;  // a half warp leaves as one
@@ -258,6 +259,8 @@ __global__ void __launch_bounds__(kWbThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  grid_wait();     // for the rows' statistics
+  grid_release();  // dQ's blocks take the SMs that run out of dK's and dV's
   ItemQueue<KvItem> queue{smem_u32(smem + L::kBar) + 256, answer, asked, wfull, wempty};
 
   if (warp < 4) {
@@ -1022,6 +1025,9 @@ __global__ void __launch_bounds__(kWbThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  // The kernel before may still run (its blocks waited for the statistics that this
+  // one reads): what follows in the stream counts on both.
+  grid_wait();
 }
 
 int padded(int S) { return (S + 127) / 128 * 128; }
@@ -1069,16 +1075,17 @@ int launch_bwd(const WindowAttnBwdArgs& a, cudaStream_t stream) {
   window_dot_kernel<<<static_cast<unsigned>((dots + 15) / 16), 256, 0, stream>>>(
       f.o, a.dout, a.ldo, f.lse, f.lengths, NL, ND, f.S, Sp, f.H, HD, dots);
   const float sl2 = f.scale * kLog2eWa;
-  window_dkdv_kernel<HD><<<static_cast<unsigned>(kv_blocks), kWbThreads, KvLayout<HD>::kSmem, stream>>>(
-      m, mdo, NL, ND, f.lengths, a.dqkv, parts, f.B, f.S, Sp, f.H, f.Hkv, plan, sl2, f.scale, f.status);
+  if (launch_over(window_dkdv_kernel<HD>, kv_blocks, kWbThreads, KvLayout<HD>::kSmem, stream, m, mdo, NL, ND,
+                  f.lengths, a.dqkv, parts, f.B, f.S, Sp, f.H, f.Hkv, plan, sl2, f.scale, f.status) != cudaSuccess ||
+      launch_over(window_dq_kernel<HD>, q_blocks, kWbThreads, DqLayout<HD>::kSmem, stream, m, mdo, NL, ND, f.lengths,
+                  a.dqkv, f.B, f.S, Sp, f.H, f.Hkv, plan.window, plan.sinks, sl2, f.scale, f.status) != cudaSuccess)
+    return 2;
   if (plan.parts > 1) {
     const int rows = (plan.sinks + 31) / 32 * 32;
     const int64_t t = static_cast<int64_t>(f.B) * f.Hkv * rows * (2 * HD / 4);
     window_sinks_kernel<<<static_cast<unsigned>((t + 255) / 256), 256, 0, stream>>>(
         parts, a.dqkv, f.S, f.H, f.Hkv, HD, rows, plan.sink_tiles, plan.parts, f.scale, t);
   }
-  window_dq_kernel<HD><<<static_cast<unsigned>(q_blocks), kWbThreads, DqLayout<HD>::kSmem, stream>>>(
-      m, mdo, NL, ND, f.lengths, a.dqkv, f.B, f.S, Sp, f.H, f.Hkv, plan.window, plan.sinks, sl2, f.scale, f.status);
   return cudaGetLastError() == cudaSuccess ? 0 : 2;
 }
 

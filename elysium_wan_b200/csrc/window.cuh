@@ -254,14 +254,18 @@ __device__ __forceinline__ void lds4(uint32_t addr, f32x2& lo, f32x2& hi) {
 // A softmax or epilogue warp's 32 rows x 64 columns (fewer in a ragged last
 // chunk: `units` 16-byte units a row, 8, 4 or 2) as bf16, written along rows
 // through its 4 KB of shared memory: 16 bytes a lane straight from its own row
-// would touch 32 lines with every store. y: the lane's row, `out` row 0 of 32.
-__device__ __forceinline__ void store_rows(const uint32_t* y, uint32_t stage, __nv_bfloat16* out, int64_t ld,
-                                           int units, int rows, int lane) {
+// would touch 32 lines with every store. stage_row: N units of the lane's
+// row, from the e-th N; store_rows: the rows, `out` row 0 of 32.
+template <int N>
+__device__ __forceinline__ void stage_row(const uint32_t* y, int e, uint32_t stage, int lane) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(stage + lane * 128 + ((e ^ (lane & 7)) << 4)),
-                 "r"(y[4 * e]), "r"(y[4 * e + 1]), "r"(y[4 * e + 2]), "r"(y[4 * e + 3])
+  for (int k = 0; k < N; ++k)
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(stage + lane * 128 + (((N * e + k) ^ (lane & 7)) << 4)),
+                 "r"(y[4 * k]), "r"(y[4 * k + 1]), "r"(y[4 * k + 2]), "r"(y[4 * k + 3])
                  : "memory");
+}
+__device__ __forceinline__ void store_rows(uint32_t stage, __nv_bfloat16* out, int64_t ld, int units, int rows,
+                                           int lane) {
   __syncwarp();
   const int lg = units == 8 ? 3 : units == 4 ? 2 : 1;
 #pragma unroll

@@ -430,24 +430,24 @@ __global__ void __launch_bounds__(kWaThreads, 1)
         __nv_bfloat16* oblk = o + ((static_cast<size_t>(a.b) * S + first + wq * 32) * H + a.h) * HD;
 #pragma unroll 1
         for (int c = 0; c < L::kChunks; ++c) {
-          uint32_t y[32];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            uint32_t v[16];  // past a ragged chunk's end: columns nobody uses
+            uint32_t v[16], y[8];  // past a ragged chunk's end: columns nobody uses
             if (mine > 0) {
               tmem_ld16(o_t + c * 64 + e * 16, v);
               tmem_wait_ld();
             }
 #pragma unroll
             for (int z = 0; z < 8; ++z)
-              y[8 * e + z] = in ? pack_bf16x2(__uint_as_float(v[2 * z]) * inv, __uint_as_float(v[2 * z + 1]) * inv) : 0u;
+              y[z] = in ? pack_bf16x2(__uint_as_float(v[2 * z]) * inv, __uint_as_float(v[2 * z + 1]) * inv) : 0u;
+            stage_row<2>(y, e, stage, lane);
           }
           if (mine > 0 && c == L::kChunks - 1) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&ofree[t]);
           }
-          store_rows(y, stage, oblk + c * 64, static_cast<int64_t>(H) * HD, HeadChunks<HD>::units(c),
+          store_rows(stage, oblk + c * 64, static_cast<int64_t>(H) * HD, HeadChunks<HD>::units(c),
                      S - first - wq * 32, lane);
         }
         if (mine > 0) ++items;

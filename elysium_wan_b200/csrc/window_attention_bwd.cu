@@ -31,8 +31,8 @@ namespace {
 // four warpgroups: producer, MMA issuer and the asking warp; epilogue; softmax of
 // each half of a tile's columns
 constexpr int kWbThreads = 512;
-// registers a thread: 64 + 96 + 2 x 176 = 4 x 128, what the launch takes
-constexpr int kWbRegsIssue = 64, kWbRegsEpilogue = 96, kWbRegsSoftmax = 176;
+// registers a thread: 56 + 104 + 2 x 176 = 4 x 128, what the launch takes
+constexpr int kWbRegsIssue = 56, kWbRegsEpilogue = 104, kWbRegsSoftmax = 176;
 constexpr int kWbWalkers = 14;  // warps that walk the queue: producer, issuer, 4 epilogue, 8 softmax
 
 // ---------------------------------------------------------------- D and lse2
@@ -220,8 +220,8 @@ __global__ void __launch_bounds__(kWbThreads, 1)
   uint64_t* pfull = bars + 13;   // the first 32 queries of each half of P^T; the rest: pfull2
   uint64_t* dpfull = bars + 14;
   uint64_t* dsfull = bars + 15;
-  uint64_t* accfull = bars + 16;
-  uint64_t* accfree = bars + 17;
+  uint64_t* accfull = bars + 16;  // dV; dK: + 11
+  uint64_t* accfree = bars + 17;  // dV; dK: + 11
   uint64_t* landed = bars + 18;  // a query tile that the producer clears
   uint64_t* drain = bars + 19;
   uint64_t* wfull = bars + 20;
@@ -240,8 +240,10 @@ __global__ void __launch_bounds__(kWbThreads, 1)
     mbar_init(pfull2, 8);
     mbar_init(dpfull, 1);
     mbar_init(dsfull, 8);
-    mbar_init(accfull, 1);
-    mbar_init(accfree, 4);
+    for (int z = 0; z < 2; ++z) {
+      mbar_init(accfull + 11 * z, 1);
+      mbar_init(accfree + 11 * z, 4);
+    }
     mbar_init(landed, 1);
     mbar_init(drain, 1);
     mbar_init(wfull, 1);
@@ -385,10 +387,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
           const bool more = t < steps;
           const int s = tn & 1, sp = s ^ 1;
           if (held) {  // dV += P^T dO
-            if (first) {
-              ok = warp_wait(accfree, (accs & 1) ^ 1, status, kStatusTimeoutTmemEmpty);
-              ++accs;
-            }
+            if (first) ok = warp_wait(accfree, (accs & 1) ^ 1, status, kStatusTimeoutTmemEmpty);
             ok = ok && warp_wait(pfull, (tn - 1) & 1, status, kStatusTimeoutTmemFull);
             tc_fence_after();
 #pragma unroll
@@ -406,6 +405,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
               }
             }
             if (ok) umma_commit_by(lead, &gempty[sp]);
+            if (ok && last) umma_commit_by(lead, accfull);
           }
           if (ok && more) {  // S^T = K Q^T
             if (t == 0) ok = warp_wait(kfull, items & 1, status, kStatusTimeoutSmemFull);
@@ -424,6 +424,10 @@ __global__ void __launch_bounds__(kWbThreads, 1)
           }
           if (ok && held) {  // dK += dS^T Q
             ok = warp_wait(dsfull, (tn - 1) & 1, status, kStatusTimeoutTmemFull);
+            if (first) {
+              ok = ok && warp_wait(accfree + 11, (accs & 1) ^ 1, status, kStatusTimeoutTmemEmpty);
+              ++accs;
+            }
             tc_fence_after();
             if (ok) {
 #pragma unroll
@@ -431,7 +435,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
                 umma_ts(lead, tmem + 384, tmem + 128 + (kk >> 2) * 64 + (kk & 3) * 8,
                         desc_at(qt_desc, sp * L::kTile + kk * 2048), IG, (!first || kk > 0) ? 1u : 0u);
               umma_commit_by(lead, &qempty[sp]);
-              if (last) umma_commit_by(lead, accfull);
+              if (last) umma_commit_by(lead, accfull + 11);
             }
           }
           if (ok && more) {  // dP^T = V dO^T
@@ -471,12 +475,6 @@ __global__ void __launch_bounds__(kWbThreads, 1)
     int items = 0;
     for (KvItem a; ok && queue.next(a, status, lane);) {
       const bool some = a.steps > 0;
-      if (some) {
-        ok = warp_wait(accfull, items & 1, status, kStatusTimeoutTmemFull);
-        if (!ok) break;
-        ++items;
-        tc_fence_after();
-      }
       const int row0 = a.k0 + wq * 32;
       // of a sinks' tile: sums of parts where these rows have a sink; else only the
       // first part has anything, their gradients
@@ -486,40 +484,48 @@ __global__ void __launch_bounds__(kWbThreads, 1)
         sum += ((((static_cast<size_t>(a.b) * Hkv + a.hk) * plan.sink_tiles + a.kt) * plan.parts + a.part) * 128 +
                 wq * 32 + lane) * (2 * HD);
 #pragma unroll 1
-      for (int z = 0; z < 2; ++z) {  // dV, then dK
+      for (int z = 0; z < 2; ++z) {  // dV, then dK: done half a step later
+        if (some) {
+          ok = warp_wait(accfull + 11 * z, items & 1, status, kStatusTimeoutTmemFull);
+          if (!ok) break;
+          tc_fence_after();
+        }
         const float mul = z ? scale : 1.0f;
         __nv_bfloat16* out = dqkv + (static_cast<int64_t>(a.b) * S + row0) * ldq + (z ? H + a.hk : H + Hkv + a.hk) * HD;
 #pragma unroll 1
         for (int c = 0; c < C::kCount; ++c) {
-          uint32_t y[32];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint32_t v[16];
-            if (some) {
-              tmem_ld16(tmem + 256 + z * 128 + lanes + c * 64 + e * 16, v);
+          for (int e = 0; e < 2; ++e) {
+            uint32_t v[32];
+            if (some && 4 * e < C::units(c)) {
+              tmem_ld32(tmem + 256 + z * 128 + lanes + c * 64 + e * 32, v);
               tmem_wait_ld();
             } else {
 #pragma unroll
-              for (int k = 0; k < 16; ++k) v[k] = 0u;
+              for (int k = 0; k < 32; ++k) v[k] = 0u;
             }
-            if (sums && 2 * e < C::units(c)) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                *reinterpret_cast<uint4*>(sum + z * HD + c * 64 + e * 16 + 4 * k) =
-                    make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+            if (e == 1 && some && c == C::kCount - 1) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(accfree + 11 * z);
             }
+            if (sums) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              y[8 * e + k] = pack_bf16x2(__uint_as_float(v[2 * k]) * mul, __uint_as_float(v[2 * k + 1]) * mul);
+              for (int k = 0; k < 8; ++k)
+                if (8 * e + k < 2 * C::units(c))
+                  *reinterpret_cast<uint4*>(sum + z * HD + c * 64 + e * 32 + 4 * k) =
+                      make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+            }
+            uint32_t y[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+              y[k] = pack_bf16x2(__uint_as_float(v[2 * k]) * mul, __uint_as_float(v[2 * k + 1]) * mul);
+            stage_row<4>(y, e, stage, lane);
           }
-          if (some && z == 1 && c == C::kCount - 1) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(accfree);
-          }
-          if (grads) store_rows(y, stage, out + c * 64, ldq, C::units(c), S - row0, lane);
+          if (grads) store_rows(stage, out + c * 64, ldq, C::units(c), S - row0, lane);
         }
       }
+      if (some) ++items;
     }
   } else {
     reg_inc<kWbRegsSoftmax>();
@@ -931,27 +937,28 @@ __global__ void __launch_bounds__(kWbThreads, 1)
       __nv_bfloat16* out = dqkv + (static_cast<int64_t>(a.b) * S + row0) * ldq + a.h * HD;
 #pragma unroll 1
       for (int c = 0; c < C::kCount; ++c) {
-        uint32_t y[32];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t v[16];
-          if (some) {
-            tmem_ld16(tmem + 384 + lanes + c * 64 + e * 16, v);
+        for (int e = 0; e < 2; ++e) {
+          uint32_t v[32];
+          if (some && 4 * e < C::units(c)) {
+            tmem_ld32(tmem + 384 + lanes + c * 64 + e * 32, v);
             tmem_wait_ld();
           } else {
 #pragma unroll
-            for (int k = 0; k < 16; ++k) v[k] = 0u;
+            for (int k = 0; k < 32; ++k) v[k] = 0u;
           }
+          if (e == 1 && some && c == C::kCount - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(accfree);
+          }
+          uint32_t y[16];
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            y[8 * e + k] = pack_bf16x2(__uint_as_float(v[2 * k]) * scale, __uint_as_float(v[2 * k + 1]) * scale);
+          for (int k = 0; k < 16; ++k)
+            y[k] = pack_bf16x2(__uint_as_float(v[2 * k]) * scale, __uint_as_float(v[2 * k + 1]) * scale);
+          stage_row<4>(y, e, stage, lane);
         }
-        if (some && c == C::kCount - 1) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(accfree);
-        }
-        store_rows(y, stage, out + c * 64, ldq, C::units(c), S - row0, lane);
+        store_rows(stage, out + c * 64, ldq, C::units(c), S - row0, lane);
       }
     }
   } else {

@@ -121,20 +121,28 @@ __device__ __forceinline__ void grads32(uint32_t* d, const uint32_t* p, F nd) {
   }
 }
 
-// 32 columns in bf16 to TMEM (16 columns from `at`).
-__device__ __forceinline__ void store32(uint32_t at, const uint32_t* v) {
+// 0 in the places of 32 packed bf16 whose bit is not set, whatever is there. A
+// mask of two bits takes one byte permute, which can spread a byte's top bit.
+__device__ __forceinline__ void keep32(uint32_t* pk, uint32_t bits) {
+  uint32_t t[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) t[j] = bits << (7 - j);
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const int b = e >> 2, j = (2 * e) & 7;
+    uint32_t m;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(m) : "r"(t[j]), "r"(t[j + 1]), "r"((8 + b) * 0x11 + (12 + b) * 0x1100));
+    pk[e] &= m;
+  }
+}
+
+// 32 columns in bf16 to TMEM (16 columns from `at`), with `mask` only those in bits.
+__device__ __forceinline__ void store32(uint32_t at, const uint32_t* v, bool mask, uint32_t bits) {
   uint32_t pk[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) pk[e] = pack_bf16x2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
+  if (mask) keep32(pk, bits);
   tmem_st16(at, pk);
-}
-
-// 0 in the places of v whose bit is not set.
-__device__ __forceinline__ void clear32(uint32_t* v, uint32_t bits) {
-  if (__all_sync(0xffffffffu, bits == 0xffffffffu)) return;
-#pragma unroll
-  for (int e = 0; e < 32; ++e)
-    if (!((bits >> e) & 1u)) v[e] = 0u;
 }
 
 // ---------------------------------------------------------------- dK, dV
@@ -573,8 +581,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
           // those of the next 32 columns, or the first -D
 #pragma unroll
           for (int e = 0; e < 8; ++e) lds4(stat + (c ? 512 : 128) + e * 16, st[2 * e], st[2 * e + 1]);
-          if (!whole) clear32(v + 32 * c, vis[c]);
-          store32(half + c * 16, v + 32 * c);
+          store32(half + c * 16, v + 32 * c, !whole, vis[c]);
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
@@ -593,8 +600,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
           }
           tmem_wait_ld();
           grads32(d, v + 32 * c, [&](int e) { return st[e]; });
-          if (!whole) clear32(d, vis[c]);  // dP of a key past the length may be NaN
-          store32(half + 128 + c * 16, d);
+          store32(half + 128 + c * 16, d, !whole, vis[c]);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -998,10 +1004,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
         tmem_ld32(s_t + 32, v + 32);
         tmem_wait_ld();
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          weights32(v + 32 * c, scale2, [&](int) { return nl2; });
-          if (!whole) clear32(v + 32 * c, vis[c]);
-        }
+        for (int c = 0; c < 2; ++c) weights32(v + 32 * c, scale2, [&](int) { return nl2; });
         ok = warp_wait(dpfull, tn & 1, status, kStatusTimeoutTmemFull);
         if (!ok) break;
         tc_fence_after();
@@ -1015,8 +1018,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           grads32(d + 32 * c, v + 32 * c, [&](int) { return nd2; });
-          if (!whole) clear32(d + 32 * c, vis[c]);  // dP of a key past the length may be NaN
-          store32(s_t + c * 16, d + 32 * c);
+          store32(s_t + c * 16, d + 32 * c, !whole, vis[c]);
         }
         tmem_wait_st();
         tc_fence_before();

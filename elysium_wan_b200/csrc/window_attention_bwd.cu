@@ -154,8 +154,8 @@ __device__ __forceinline__ void store32(uint32_t at, const uint32_t* v, bool mas
 // of S^T and dP^T as bf16 and are A operands from there, which takes a third of
 // the operand traffic off shared memory. The epilogue warps empty the
 // accumulators while the next block's steps begin.
-// TMEM: S^T | dP^T | dV | dK (128 columns each). Shared memory: K, V, two
-// stages of Q, dO and the statistics.
+// TMEM: S^T | dP^T | dV | dK (128 columns each). Shared memory: K, V, Q and dO of
+// two steps, the statistics of four.
 struct KvPlan {
   int window, sinks;  // bounded by S
   int sink_tiles;     // key tiles with a sink
@@ -167,8 +167,8 @@ template <int HD>
 struct KvLayout {
   static constexpr int kChunks = HeadChunks<HD>::kCount;
   static constexpr uint32_t kTile = kChunks * kWaChunk;
-  static constexpr uint32_t kK = 0, kV = kTile, kQ = 2 * kTile, kO = 4 * kTile, kStat = 6 * kTile;
-  static constexpr uint32_t kStage = kStat + 2048, kBar = kStage + 4 * 4096;
+  static constexpr uint32_t kK = 0, kV = kTile, kQ = 2 * kTile, kStat = 6 * kTile;  // kQ: Q and dO
+  static constexpr uint32_t kStage = kStat + 4096, kBar = kStage + 4 * 4096;
   static constexpr int kSmem = static_cast<int>(kBar) + 512 + 1024;
 };
 
@@ -290,9 +290,10 @@ __global__ void __launch_bounds__(kWbThreads, 1)
           const uint32_t ph = ((tn >> 1) & 1) ^ 1;
           const int h = a.hk * rep + t / a.nqs, i = a.i0 + t % a.nqs;
           const bool patch = i == clear;
-          uint8_t* sq = smem + L::kQ + s * L::kTile;
-          uint8_t* sg = smem + L::kO + s * L::kTile;
-          uint8_t* st = smem + L::kStat + s * 1024;
+          // dO of two steps before is done with before its Q is: Q takes its place
+          uint8_t* sq = smem + L::kQ + (s + (tn & 2)) * L::kTile;
+          uint8_t* sg = smem + L::kQ + (s + (~tn & 2)) * L::kTile;
+          uint8_t* st = smem + L::kStat + (tn & 3) * 1024;
           if (t == 0) {
             ok = warp_wait(kempty, (items & 1) ^ 1, status, kStatusTimeoutSmemEmpty);
             if (!ok) break;
@@ -303,9 +304,9 @@ __global__ void __launch_bounds__(kWbThreads, 1)
             }
             ++kn;
           }
-          ok = warp_wait(&qempty[s], ph, status, kStatusTimeoutSmemEmpty);
-          // a cleared step comes whole: its dO stage has to be free as well
-          if (patch) ok = ok && warp_wait(&gempty[s], ph, status, kStatusTimeoutSmemEmpty);
+          ok = warp_wait(&gempty[s], ph, status, kStatusTimeoutSmemEmpty);
+          // a cleared step comes whole: the place of its dO has to be free as well
+          if (patch) ok = ok && warp_wait(&qempty[s], ph, status, kStatusTimeoutSmemEmpty);
           if (!ok) break;
           uint64_t* bar = patch ? landed : &qfull[s];
           if (lane == 0) {
@@ -330,7 +331,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
             }
           }
           if (!patch) {
-            ok = ok && warp_wait(&gempty[s], ph, status, kStatusTimeoutSmemEmpty);
+            ok = ok && warp_wait(&qempty[s], ph, status, kStatusTimeoutSmemEmpty);
             if (!ok) break;
             bar = &gfull[s];
             if (lane == 0) mbar_arrive_expect_tx(bar, L::kTile);
@@ -379,9 +380,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
       const uint64_t v_desc = sdesc_sw128(smem_u32(smem + L::kV), 16, 1024);
       // Q and dO as K-major (scores) and MN-major (gradients) operands
       const uint64_t q_desc = sdesc_sw128(smem_u32(smem + L::kQ), 16, 1024);
-      const uint64_t g_desc = sdesc_sw128(smem_u32(smem + L::kO), 16, 1024);
       const uint64_t qt_desc = sdesc_sw128(smem_u32(smem + L::kQ), kWaChunk, 1024);
-      const uint64_t gt_desc = sdesc_sw128(smem_u32(smem + L::kO), kWaChunk, 1024);
       bool ok = true;
       int items = 0, tn = 0, accs = 0;
       // the step before: to be finished, the first or last of its block
@@ -394,6 +393,9 @@ __global__ void __launch_bounds__(kWbThreads, 1)
         for (int t = 0; t < max(steps, 1) && ok; ++t) {
           const bool more = t < steps;
           const int s = tn & 1, sp = s ^ 1;
+          // the places of this step's Q and of the step before's; the other two are dO's
+          const uint32_t q_at = (s + (tn & 2)) * L::kTile, qp_at = (sp + ((tn - 1) & 2)) * L::kTile;
+          const uint32_t g_at = (s + (~tn & 2)) * L::kTile, gp_at = (sp + (~(tn - 1) & 2)) * L::kTile;
           if (held) {  // dV += P^T dO
             if (first) ok = warp_wait(accfree, (accs & 1) ^ 1, status, kStatusTimeoutTmemEmpty);
             ok = ok && warp_wait(pfull, (tn - 1) & 1, status, kStatusTimeoutTmemFull);
@@ -409,7 +411,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
                 for (int kk = 0; kk < 8; ++kk)
                   if (((kk >> 1) & 1) == z)
                     umma_ts(lead, tmem + 256, tmem + (kk >> 2) * 64 + (kk & 3) * 8,
-                            desc_at(gt_desc, sp * L::kTile + kk * 2048), IG, (!first || kk > 0) ? 1u : 0u);
+                            desc_at(qt_desc, gp_at + kk * 2048), IG, (!first || kk > 0) ? 1u : 0u);
               }
             }
             if (ok) umma_commit_by(lead, &gempty[sp]);
@@ -425,7 +427,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
 #pragma unroll
                 for (int kk = 0; kk < C::steps(c); ++kk)
                   umma_ss(lead, tmem, desc_at(k_desc, c * kWaChunk + kk * 32),
-                          desc_at(q_desc, s * L::kTile + c * kWaChunk + kk * 32), IS, (c > 0 || kk > 0) ? 1u : 0u);
+                          desc_at(q_desc, q_at + c * kWaChunk + kk * 32), IS, (c > 0 || kk > 0) ? 1u : 0u);
               umma_commit_by(lead, sfull);
               if (t == steps - 1) umma_commit_by(lead, kempty);
             }
@@ -441,7 +443,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
 #pragma unroll
               for (int kk = 0; kk < 8; ++kk)
                 umma_ts(lead, tmem + 384, tmem + 128 + (kk >> 2) * 64 + (kk & 3) * 8,
-                        desc_at(qt_desc, sp * L::kTile + kk * 2048), IG, (!first || kk > 0) ? 1u : 0u);
+                        desc_at(qt_desc, qp_at + kk * 2048), IG, (!first || kk > 0) ? 1u : 0u);
               umma_commit_by(lead, &qempty[sp]);
               if (last) umma_commit_by(lead, accfull + 11);
             }
@@ -456,7 +458,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
 #pragma unroll
                 for (int kk = 0; kk < C::steps(c); ++kk)
                   umma_ss(lead, tmem + 128, desc_at(v_desc, c * kWaChunk + kk * 32),
-                          desc_at(g_desc, s * L::kTile + c * kWaChunk + kk * 32), IS, (c > 0 || kk > 0) ? 1u : 0u);
+                          desc_at(q_desc, g_at + c * kWaChunk + kk * 32), IS, (c > 0 || kk > 0) ? 1u : 0u);
               umma_commit_by(lead, dpfull);
               if (t == steps - 1) umma_commit_by(lead, vempty);
             }
@@ -552,7 +554,7 @@ __global__ void __launch_bounds__(kWbThreads, 1)
         // the statistics, and this step's mask, before the scores are there
         ok = warp_wait(&qfull[s], (tn >> 1) & 1, status, kStatusTimeoutSmemFull);
         if (!ok) break;
-        const uint32_t stat = smem_u32(smem + L::kStat) + s * 1024 + g * 256;
+        const uint32_t stat = smem_u32(smem + L::kStat) + (tn & 3) * 1024 + g * 256;
         f32x2 st[16];
 #pragma unroll
         for (int e = 0; e < 8; ++e) lds4(stat + e * 16, st[2 * e], st[2 * e + 1]);

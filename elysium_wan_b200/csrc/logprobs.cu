@@ -27,9 +27,10 @@
 // Rows may start anywhere (an odd vocabulary): vectors are aligned in memory
 // and the two at the ends of the row are read element by element.
 //
-// The gradient is one read and one write. fp32 logits are bound by memory (fp32,
-// 4096 x 50257 forward: 0.9 of the measured copy rate); bf16 ones by the
-// instructions for each logit, hence the packed pairs.
+// The gradient is one read and one write. fp32 logits are bound by memory: 2048 x
+// 50257 takes 74 us forward (5.5 TB/s, 0.86 of the measured copy rate) and 114 us
+// for a bf16 gradient (0.84); bf16 logits by the instructions for each of them, hence the
+// packed pairs.
 #include "common.cuh"
 #include "kernels.h"
 #include "pairs.cuh"

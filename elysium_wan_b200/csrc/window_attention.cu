@@ -31,6 +31,15 @@
 // Rows past a sequence's end: boxes of the 3D tensor map read zeros past S; the
 // V tile that holds the end of a shorter sequence is cleared from there on by
 // the producer, so that 0 x NaN cannot reach a sum. Every wait is bounded.
+//
+// P enters the second product as bf16, its row sums are of the fp32 weights.
+//
+// 8192 tokens, 32 heads of 128 on 8, window 1024, 4 sinks: 152 to 169 us (the clock
+// is 1.6 to 1.9 GHz by power), 780 TFLOP/s of the visible pairs; the tensor pipe is
+// busy for 47% of it. Of a period of about 3050 cycles for two subtiles, 2048 are
+// tensor work and 1980 softmax (8 exponentials of 32 on the FMA pipe); the rest is the
+// hand-over between them. All exponentials on the special-function unit: 3600
+// cycles; 16 softmax warps of half a row each: spills, 265 us for 214 then.
 #include "common.cuh"
 #include "gemm.h"
 #include "kernels.h"

@@ -14,7 +14,11 @@
 // mma fragments, with a softmax of their own each (running maximum and sum in fp32);
 // warps join in shared memory, CTAs through distributed shared memory, both in a
 // fixed order. Only other warps cover a warp's loads (4 to 8 KB a group), so CTAs
-// are of four warps and several share an SM.
+// are of four warps and several share an SM. 8 answers of 40 heads x 128 over 4160
+// rows: 152 us, 4.5 TB/s (0.69 of the measured copy rate). Rings of three groups a
+// warp in shared memory, filled by asynchronous copies, took 171 to 232: they leave
+// room for two CTAs an SM, and whole rounds of CTAs then cost more than the loads in
+// flight gain.
 //
 // Both products have the 16 rows (or 16 columns of the head) as the m of m16n8k16 and
 // the query heads as its n: S^T = K Q^T and O^T = V^T P^T. The contraction order

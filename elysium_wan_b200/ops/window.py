@@ -9,6 +9,8 @@ Tensors are those of the full attention: rows of q (H heads) | k (Hkv) | v
 (Hkv), hd columns a head. The GPU kernels take hd 64, 80, 96 and 128, any
 number of rows, and rows that are strided as long as they are 16-byte aligned.
 What lies in rows at or past a sequence's length is never used, NaN included.
+Inside a sequence values have to be finite: the kernels multiply whole tiles of
+128 keys, where a masked weight of 0 times an infinity is NaN.
 """
 
 from __future__ import annotations

@@ -10,6 +10,9 @@ attn_fwd, attn_bwd, ln_fwd, ln_bwd, ce, adamw, embed_bwd, head_gemm (the 50257-w
 logits GEMM, fp32 out), head_lse (the fused logits GEMM + cross-entropy: LSE epilogue and
 finalize), head_fwd (LN + fused logits / CE of the head entry), head_bwd
 (its forward, backward and W).
+For long texts, at sizes of their own: window_fwd, window_bwd (8192 tokens, 32 heads on 8
+key-value heads, window 1024, 4 sinks), window_step (8 answers of 40 heads, window 4096),
+logprobs, logprobs_bwd (2048 rows of 50257 fp32 logits), dropout, dropout_bwd (16384 x 5120 bf16).
 """
 
 from __future__ import annotations
@@ -136,6 +139,32 @@ def build(op):
         m, v = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
         pb = torch.empty(n, dtype=torch.bfloat16, device="cuda")
         return (lambda: ops.adamw(p, m, v, g, pb, 1e-4, 0.9, 0.95, 1e-8, 0.0, 1)), None, n * 30
+    if op in ("window_fwd", "window_bwd"):
+        S, h, hkv, hd, w, k = 8192, 32, 8, 128, 1024, 4
+        qkv, do, kw = _bf(S, (h + 2 * hkv) * hd), _bf(S, h * hd), dict(window=w, sinks=k)
+        o, lse = ops.window_attention_fwd(qkv, 1, S, h, hd, hkv, **kw)
+        pairs = h * (S * w - w * (w - 1) // 2 + k * (S - w) - k * (k - 1) // 2)
+        if op == "window_fwd":
+            return (lambda: ops.window_attention_fwd(qkv, 1, S, h, hd, hkv, **kw)), 4.0 * pairs * hd, None
+        return (lambda: ops.window_attention_bwd(qkv, o, do, lse, 1, S, h, hd, hkv, **kw)), \
+            10.0 * pairs * hd, None
+    if op == "window_step":
+        b, h, hd, w, k = 8, 40, 128, 4096, 64
+        qkv, cache = _bf(b, 3 * h * hd), _bf(b, w + k, 2 * h * hd)
+        pos = torch.full((b,), 2 * w, dtype=torch.int64, device="cuda")
+        return (lambda: ops.window_attention_step(qkv, cache, pos, h, hd, window=w, sinks=k)), None, \
+            b * (w + k) * 4 * h * hd
+    if op in ("logprobs", "logprobs_bwd"):
+        logits, tgt = torch.randn(T, V, device="cuda"), torch.randint(0, V, (T,), device="cuda")
+        if op == "logprobs":
+            return (lambda: ops.token_logprobs(logits, V, tgt)), None, T * V * 4
+        r, g = ops.token_logprobs(logits, V, tgt), torch.randn(T, device="cuda")
+        return (lambda: ops.token_logprobs_bwd(logits, V, tgt, r.lse, r.entropy, g, g)), None, T * V * 6
+    if op in ("dropout", "dropout_bwd"):
+        x, r = _bf(8 * T, D), _bf(8 * T, D)
+        if op == "dropout":
+            return (lambda: ops.dropout_add(x, r, 0.1, 1, 2)), None, 8 * T * D * 6
+        return (lambda: ops.dropout_bwd(x, 0.1, 1, 2)), None, 8 * T * D * 4
     if op == "embed_bwd":
         idx = torch.randint(0, V, (1, T), device="cuda")
         dx = _bf(T, D)

@@ -773,7 +773,8 @@ __global__ void __launch_bounds__(kWbThreads, 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {  // padded rows: -inf, 0
           const uint32_t to = smem_u32(smem + L::kStat) + (i * 32 + lane) * 8;
-          asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(NL[at + 32 * i]), "f"(ND[at + 32 * i])
+          asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(__ldcg(NL + at + 32 * i)),
+                       "f"(__ldcg(ND + at + 32 * i))
                        : "memory");
         }
         return a;

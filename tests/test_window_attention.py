@@ -256,6 +256,60 @@ def test_gpu_other_stream_and_wide_batch(cuda):
     assert torch.equal(a[0], b[0])
 
 
+def _calls(cuda):
+    """Shapes whose backward takes 3 launches or 4 (a split sinks' tile), and their inputs."""
+    for B, S, H, hd, Hkv, window, sinks in ((1, 1500, 4, 128, 2, 100, 4), (2, 700, 3, 64, 3, 300, 0),
+                                            (1, 77, 4, 80, 2, 32, 4)):
+        yield (B, S, H, hd, Hkv), dict(window=window, sinks=sinks), inputs(B, S, H, hd, Hkv, cuda)
+
+
+@pytest.mark.gpu
+def test_gpu_back_to_back(cuda):
+    """Launches that overlap inside one call must not reach into the next one's
+    workspace, or be overtaken by what reads the gradient."""
+    calls = list(_calls(cuda))
+    want, got = [], []
+    for shape, kw, (qkv, dout) in calls:
+        o, lse = ops.window_attention_fwd(qkv, *shape, **kw)
+        torch.cuda.synchronize()
+        want.append(ops.window_attention_bwd(qkv, o, dout, lse, *shape, **kw))
+        torch.cuda.synchronize()
+    for _ in range(20):
+        for shape, kw, (qkv, dout) in calls:
+            o, lse = ops.window_attention_fwd(qkv, *shape, **kw)
+            d = ops.window_attention_bwd(qkv, o, dout, lse, *shape, **kw)
+            got.append(d.clone())
+            d.fill_(float("nan"))  # follows the gradient's last launch, not its first
+            del o, lse, d
+    torch.cuda.synchronize()
+    for i, d in enumerate(got):
+        assert torch.equal(d, want[i % len(want)])
+
+
+@pytest.mark.gpu
+def test_gpu_in_a_graph(cuda):
+    for shape, kw, (qkv, dout) in _calls(cuda):
+        def both():
+            o, lse = ops.window_attention_fwd(qkv, *shape, **kw)
+            return o, lse, ops.window_attention_bwd(qkv, o, dout, lse, *shape, **kw)
+
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            both()
+        torch.cuda.current_stream().wait_stream(s)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = both()
+        qkv.copy_(torch.randn_like(qkv))  # a replay reads what is there then
+        for t in out:
+            t.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, both()):
+            assert torch.equal(a, b)
+
+
 @pytest.mark.gpu
 def test_gpu_refusals(cuda):
     B, S, H, hd, Hkv = 2, 5, 4, 64, 2

@@ -586,10 +586,11 @@ __global__ void __launch_bounds__(kWbThreads, 1)
         tc_fence_after();
         uint32_t v[64];
         tmem_ld32(half, v);
-        tmem_ld32(half + 32, v + 32);
         tmem_wait_ld();
+        tmem_ld32(half + 32, v + 32);  // under the first 32 columns' weights
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
+          if (c == 1) tmem_landed32(v + 32);
           weights32(v + 32 * c, scale2, [&](int e) { return st[e]; });
           // those of the next 32 columns, or the first -D
 #pragma unroll
@@ -1018,22 +1019,26 @@ __global__ void __launch_bounds__(kWbThreads, 1)
         }
         uint32_t v[64];
         tmem_ld32(s_t, v);
-        tmem_ld32(s_t + 32, v + 32);
         tmem_wait_ld();
-#pragma unroll
-        for (int c = 0; c < 2; ++c) weights32(v + 32 * c, scale2, [&](int) { return nl2; });
+        tmem_ld32(s_t + 32, v + 32);  // under the first 32 columns' weights
+        weights32(v, scale2, [&](int) { return nl2; });
+        tmem_landed32(v + 32);
+        weights32(v + 32, scale2, [&](int) { return nl2; });
         ok = warp_wait(dpfull, tn & 1, status, kStatusTimeoutTmemFull);
         if (!ok) break;
         tc_fence_after();
         uint32_t d[64];
         tmem_ld32(half + 256, d);
-        tmem_ld32(half + 256 + 32, d + 32);
         tmem_wait_ld();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(dpfree);
+        tmem_ld32(half + 256 + 32, d + 32);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
+          if (c == 1) {
+            tmem_landed32(d + 32);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(dpfree);
+          }
           grads32(d + 32 * c, v + 32 * c, [&](int) { return nd2; });
           store32(s_t + c * 16, d + 32 * c, !whole, vis[c]);
         }

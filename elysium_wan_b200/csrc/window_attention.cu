@@ -480,12 +480,14 @@ int launch_fwd(const WindowAttnArgs& a, cudaStream_t stream) {
   CUtensorMap map;
   const uint64_t width = static_cast<uint64_t>(a.H + 2 * a.Hkv) * HD;
   if (!tma_map_bf16_3d(&map, a.qkv, width, a.S, a.B, a.ldq, 64, 128)) return 1;
-  static bool attr = false;
-  if (!attr) {
+  static bool attr[64] = {false};  // by device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!attr[dev & 63]) {
     if (cudaFuncSetAttribute(window_fwd_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              L::kSmem) != cudaSuccess)
       return 2;
-    attr = true;
+    attr[dev & 63] = true;
   }
   const int64_t total = static_cast<int64_t>(a.H) * ((a.S + 255) / 256) * a.B;
   if (total > 0x7fffffff) return 1;

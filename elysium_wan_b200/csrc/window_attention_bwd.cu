@@ -1084,8 +1084,10 @@ int launch_bwd(const WindowAttnBwdArgs& a, cudaStream_t stream) {
   if (!tma_map_bf16_3d(&m, f.qkv, width, f.S, f.B, f.ldq, 64, 128) ||
       !tma_map_bf16_3d(&mdo, a.dout, owidth, f.S, f.B, a.ldo, 64, 128))
     return 1;
-  static bool attr = false;
-  if (!attr) {
+  static bool attr[64] = {false};  // by device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!attr[dev & 63]) {
     if (cudaFuncSetAttribute(window_dkdv_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              KvLayout<HD>::kSmem) !=
             cudaSuccess ||
@@ -1093,7 +1095,7 @@ int launch_bwd(const WindowAttnBwdArgs& a, cudaStream_t stream) {
                              DqLayout<HD>::kSmem) !=
             cudaSuccess)
       return 2;
-    attr = true;
+    attr[dev & 63] = true;
   }
   const int64_t cells = static_cast<int64_t>(f.B) * f.H * Sp;
   const int64_t units = plan.sink_tiles * plan.parts + Sp / 128 - plan.sink_tiles;

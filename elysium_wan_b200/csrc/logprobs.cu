@@ -442,7 +442,7 @@ constexpr int kLgThreads = 256;
 constexpr int kLgChunk = 4096;  // columns of a block
 
 struct LpRow {
-  f32x2 minus_lse, A, B;
+  f32x2 minus_lse, shift, A, B;
   float gl;
   int t;  // -1: none given
   __device__ __forceinline__ LpRow(int64_t r, int V, const int64_t* targets, const float* lse, const float* entropy,
@@ -456,6 +456,11 @@ struct LpRow {
     // no finite logit: every p is 0, as an lse of +inf makes it
     const float minus = z == -INFINITY ? -INFINITY : -z;
     minus_lse = pair2(minus, minus);
+    // From 2^30 on (a row that a mask of the type's lowest value took whole) lse
+    // is the largest logit itself, ln s lost in its rounding, and lower ones lie at
+    // least 64 below: k equal ones have p = 1 / k each, and their entropy is ln k.
+    const float lost = fabsf(z) >= 1073741824.f && fabsf(z) < INFINITY ? -entropy[r] * kLog2eLp : 0.f;
+    shift = pair2(lost, lost);
     A = pair2(a, a);
     B = pair2(b, b);
   }
@@ -466,7 +471,7 @@ struct LpRow {
 #pragma unroll
     for (int e = 0; e < n; e += 2) {
       float u0, u1;
-      unpair2(mul2(add2(pair2(f[e], f[e + 1]), minus_lse), pair2(kLog2eLp, kLog2eLp)), u0, u1);
+      unpair2(fma2(add2(pair2(f[e], f[e + 1]), minus_lse), pair2(kLog2eLp, kLog2eLp), shift), u0, u1);
       u0 = max_nan(u0, kFloorLp);
       u1 = max_nan(u1, kFloorLp);
       unpair2(mul2(pair2(ex2_lp(u0), ex2_lp(u1)), fma2(B, pair2(u0, u1), A)), f[e], f[e + 1]);

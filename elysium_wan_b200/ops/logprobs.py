@@ -73,8 +73,10 @@ def token_logprobs_bwd(logits, V: int, targets, lse, entropy, g_logp=None, g_ent
 
     lse and entropy come from token_logprobs on the same logits; probabilities
     are e^(x - lse), so their relative error is that of the fp32 lse, |lse| /
-    2**24. ld_grad is
-    V rounded up to 8 unless given (the row length that the GEMMs read through
+    2**24. Where lse is past 2**30 in size (a row masked whole with the type's
+    lowest value) the largest logits, which are equal there, share the
+    probability: e^-entropy each. ld_grad is V rounded up to 8 unless given (the
+    row length that the GEMMs read through
     TMA); out_dtype is bf16 unless given (fp32 on the host path).
     """
     if ld_grad is None:
@@ -86,6 +88,8 @@ def token_logprobs_bwd(logits, V: int, targets, lse, entropy, g_logp=None, g_ent
         raise ValueError("ld_grad must be at least V")
     x = logits[:, :V].float()
     u = x - torch.where(lse == -math.inf, math.inf, lse)[:, None]
+    lost = (lse.abs() >= 2.0**30) & torch.isfinite(lse)  # lse is the largest logit itself
+    u = u - torch.where(lost, entropy, 0.0)[:, None]
     p = torch.exp(u)
     zero = torch.zeros_like(lse)
     t = targets.reshape(-1) if targets is not None else torch.full(lse.shape, -1)

@@ -106,6 +106,47 @@ def test_host_gradient_against_formula_and_differences():
         assert abs((f[0] - f[1]) / 2e-3 - d[row, col]) < 5e-5
 
 
+def lowest_rows(dtype, V, device):
+    """Rows of the type's lowest value alone, with ties at a higher one, and their p."""
+    low = torch.finfo(dtype).min
+    x = torch.full((4, V), low, dtype=dtype, device=device)
+    x[1, 3:V:7] = low / 2
+    x[2, V - 1] = -1.0  # an ordinary row under a mask
+    x[3] = low / 4
+    p = (x == x.amax(1, keepdim=True)).double()
+    return x, p / p.sum(1, keepdim=True)
+
+
+def check_lowest(dtype, V, device, ld):
+    x, p = lowest_rows(dtype, V, device)
+    if ld != V:
+        x = torch.nn.functional.pad(x, (0, ld - V))
+    t = torch.tensor([5, 3, V - 1, -1], device=device)
+    gl = torch.tensor([0.7, -1.3, 2.0, 1.0], device=device)
+    ge = torch.tensor([0.5, 1.1, -0.4, 3.0], device=device)
+    r = ops.token_logprobs(x, V, t)
+    d = ops.token_logprobs_bwd(x, V, t, r.lse, r.entropy, gl, ge, out_dtype=torch.float32)
+    g = torch.where(t >= 0, gl, 0.0).double()
+    # equal probabilities: log p + H = 0, so the entropy's gradient is 0
+    want = (-g[:, None] * p).scatter_add(1, t.clamp(min=0)[:, None], g[:, None])
+    # p comes from an entropy of at most 11, in fp32 a few units of 2^-21 off; so does the
+    # entropy's term p ge (log p + H). At the target p is taken from 1 in fp32.
+    tol = 1e-5 * (g.abs() + ge.double().abs())[:, None] * p + 2e-7 * g.abs()[:, None] * (want.abs() > p)
+    assert bool(((d[:, :V].double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_host_gradient_of_rows_at_the_lowest_value(dtype):
+    check_lowest(dtype, 300, "cpu", 300)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V,ld", [(300, 300), (50257, 50257), (40000, 40008)])
+def test_gpu_gradient_of_rows_at_the_lowest_value(cuda, dtype, V, ld):
+    check_lowest(dtype, V, cuda, ld)
+
+
 def test_refusals_host():
     x, t = logits(3, 8, 8, torch.float32)
     for kw in (dict(V=9), dict(V=0), dict(V=8, top=9), dict(V=8, top=-1)):
